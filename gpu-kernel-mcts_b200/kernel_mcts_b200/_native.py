@@ -1,4 +1,5 @@
-"""ctypes binding of libkmcts_gemm_sm100.so (C ABI in include/kmcts_gemm.h).
+"""ctypes binding of libkmcts_gemm_sm100.so (C ABI in include/kmcts_gemm.h
+and include/kmcts_grouped.h).
 
 There is no fallback: if the library is missing or fails to load, every call
 raises :class:`NativeLibraryError`.
@@ -60,7 +61,11 @@ TAIL_SPLIT_K = 3
 
 INPUTS = {"uniform": 0, "randn": 1, "int": 2}
 
-#: Every symbol include/kmcts_gemm.h declares.
+# kmcts_grouped.h
+GROUPED_ZERO_REST = 1
+TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
+
+#: Every symbol the headers under include/ declare.
 EXPORTED_SYMBOLS = (
     "kmcts_default_config",
     "kmcts_select_config",
@@ -83,6 +88,11 @@ EXPORTED_SYMBOLS = (
     "kmcts_copy_2d",
     "kmcts_bf16_gemm_allgather",
     "kmcts_selftest_bounded_wait",
+    "kmcts_bf16_grouped_gemm",
+    "kmcts_bf16_grouped_wgrad",
+    "kmcts_mxfp4_quantize",
+    "kmcts_mxfp4_dequantize",
+    "kmcts_mxfp4_gemm",
 )
 
 
@@ -237,6 +247,17 @@ def load() -> ctypes.CDLL:
         lib.kmcts_bf16_gemm_host.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, ctypes.POINTER(GemmConfig),
                                              i32, vp, vp]
         lib.kmcts_bf16_gemm_host.restype = i32
+        lib.kmcts_bf16_grouped_gemm.argtypes = [vp, i64, vp, i64, i64, i32, vp, i64, vp, i32, i32, i32, i32, i32, i32,
+                                                vp, vp]
+        lib.kmcts_bf16_grouped_wgrad.argtypes = [vp, i64, vp, i64, vp, i64, i64, i32, i32, vp, i32, i32, i32, i32, i32,
+                                                 vp, vp]
+        lib.kmcts_mxfp4_quantize.argtypes = [vp, i32, i64, vp, i64, vp, i64, i64, i32, vp]
+        lib.kmcts_mxfp4_dequantize.argtypes = [vp, i64, vp, i64, vp, i32, i64, i64, i32, vp]
+        lib.kmcts_mxfp4_gemm.argtypes = [vp, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, i64, vp, i32, i32, i32, i32,
+                                         i32, i32, vp, vp]
+        for name in ("kmcts_bf16_grouped_gemm", "kmcts_bf16_grouped_wgrad", "kmcts_mxfp4_quantize",
+                     "kmcts_mxfp4_dequantize", "kmcts_mxfp4_gemm"):
+            getattr(lib, name).restype = i32
         _lib = lib
         return lib
 

@@ -1,7 +1,7 @@
 """Builds the native parts of kernel_mcts_b200 in-tree with nvcc (sm_100a).
 
 Outputs (git-ignored, shipped with the source tree):
-  _lib/libkmcts_gemm_sm100.so   the C-ABI GEMM library (include/kmcts_gemm.h)
+  _lib/libkmcts_gemm_sm100.so   the C-ABI library (include/kmcts_gemm.h, kmcts_grouped.h)
   _lib/kmcts_bf16_eval          the evaluation harness executable built on it
 
 Run as ``python -m kernel_mcts_b200.build`` (with gpu-kernel-mcts_b200/ on
@@ -33,7 +33,9 @@ COMMON_FLAGS = ["-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS, f"-I{INCLUDE}", f
 
 LIBRARY_SOURCES = ("gemm_tcgen05.cu", "gemm_tcgen05_pair.cu", "gemm_tcgen05_stream.cu", "gemm_simt.cu", "compare.cu",
                    "capi.cu", "ipc.cu", "selftest.cu", "workspace.cu", "host_gemm.cu")
+GROUPED_SOURCES = ("grouped_api.cu", "grouped_simt.cu", "mxfp4_quantize.cu")
 HEADERS = ("ptx_sm100.cuh", "gemm_common.cuh", "kmcts_internal.h")
+GROUPED_HEADERS = ("grouped_common.cuh", "grouped_internal.h")
 
 
 def nvcc() -> str:
@@ -64,11 +66,12 @@ def build_library(verbose: bool = False) -> Path:
     headers = [CSRC / h for h in HEADERS] + [INCLUDE / "kmcts_gemm.h"]
     jobs = []
     objects = []
-    for name in LIBRARY_SOURCES:
+    grouped_headers = [*headers, *(CSRC / h for h in GROUPED_HEADERS), INCLUDE / "kmcts_grouped.h"]
+    for name in (*LIBRARY_SOURCES, *GROUPED_SOURCES):
         src = CSRC / name
         obj = OBJ_DIR / (Path(name).stem + ".o")
         objects.append(obj)
-        if _stale(obj, [src, *headers, Path(__file__)]):
+        if _stale(obj, [src, *(grouped_headers if name in GROUPED_SOURCES else headers), Path(__file__)]):
             jobs.append([nvcc(), *COMMON_FLAGS, "-Xcompiler", "-fPIC", "-c", str(src), "-o", str(obj)])
     if jobs:
         with concurrent.futures.ThreadPoolExecutor(max_workers=len(jobs)) as pool:

@@ -1,0 +1,222 @@
+// MXFP4 quantisation and its inverse.  Both are one pass over memory: a thread
+// holds 8 consecutive elements, so four neighbouring lanes hold one block of
+// 32 and find its largest magnitude with two shuffles; nothing is read twice.
+// Bound by HBM: 2 + 17/32 bytes an element each way for BF16.
+#include "grouped_common.cuh"
+
+namespace kmcts {
+namespace {
+
+using grouped::e8m0_value;
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 8;  // elements a thread holds: a quarter of a block
+
+template <int TYPE>
+struct Element;
+template <>
+struct Element<KMCTS_TYPE_BF16> {
+    using type = __nv_bfloat16;
+    static __device__ float to_float(type v) { return __bfloat162float(v); }
+    static __device__ type from_float(float v) { return __float2bfloat16_rn(v); }
+};
+template <>
+struct Element<KMCTS_TYPE_FP16> {
+    using type = __half;
+    static __device__ float to_float(type v) { return __half2float(v); }
+    static __device__ type from_float(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Element<KMCTS_TYPE_FP32> {
+    using type = float;
+    static __device__ float to_float(type v) { return v; }
+    static __device__ type from_float(float v) { return v; }
+};
+
+template <int TYPE>
+struct alignas(16) Chunk {
+    typename Element<TYPE>::type v[kChunk];
+};
+
+// Two FP32 values to two E2M1 codes, round to nearest even, saturating at 6;
+// `lo` in the low half of the byte.
+__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
+    uint32_t out;
+    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\tcvt.u32.u8 %0, b;\n\t}"
+        : "=r"(out)
+        : "f"(lo), "f"(hi));
+    return out;
+}
+
+// Rows of a block, so that a block has a few thousand elements whatever K is.
+// Chunk i of the block is chunk i % per_row of its row i / per_row.
+template <int TYPE, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads)
+    mxfp4_quantize_kernel(const typename Element<TYPE>::type* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
+                          int64_t ldc, uint8_t* __restrict__ scales, int64_t lds, int64_t rows, unsigned per_row,
+                          unsigned rows_per_block) {
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
+    const unsigned here = static_cast<unsigned>(min(static_cast<int64_t>(rows_per_block), rows - row0));
+    const unsigned total = here * per_row;
+    // per_row is a multiple of 4, so a block's four lanes take the loop together.
+    for (unsigned i = threadIdx.x; i < total; i += kThreads) {
+        const unsigned r = i / per_row, c = i - r * per_row;
+        const auto* src = x + (row0 + r) * ldx + static_cast<int64_t>(c) * kChunk;
+        float v[kChunk];
+        if constexpr (ALIGNED) {
+            const Chunk<TYPE> in = *reinterpret_cast<const Chunk<TYPE>*>(src);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) v[j] = Element<TYPE>::to_float(in.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) v[j] = Element<TYPE>::to_float(src[j]);
+        }
+        // Magnitudes compare as integers, and a NaN is larger than infinity.
+        uint32_t largest = 0;
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);
+        const uint32_t quad = 0xfu << (threadIdx.x & 28);
+        largest = max(largest, __shfl_xor_sync(quad, largest, 1));
+        largest = max(largest, __shfl_xor_sync(quad, largest, 2));
+        // floor(log2) is the exponent field less 127 (a subnormal's is 0, and
+        // below the smallest scale either way); E2M1's largest exponent is 2.
+        const uint32_t field = largest >> 23;
+        const uint32_t scale = field == 255 ? 255 : field > 2 ? field - 2 : 0;
+        // 1 / scale = 2^(127 - scale): exact, normal for every scale there is.
+        const float inverse = __uint_as_float(scale == 255 ? 0u : (254 - scale) << 23);
+        uint32_t packed = 0;
+#pragma unroll
+        for (int j = 0; j < kChunk; j += 2) packed |= e2m1x2(v[j] * inverse, v[j + 1] * inverse) << (4 * j);
+        uint8_t* dst = codes + (row0 + r) * ldc + static_cast<int64_t>(c) * (kChunk / 2);
+        if constexpr (ALIGNED) {
+            *reinterpret_cast<uint32_t*>(dst) = packed;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[j] = static_cast<uint8_t>(packed >> (8 * j));
+        }
+        if ((c & 3) == 0) scales[(row0 + r) * lds + c / 4] = static_cast<uint8_t>(scale);
+    }
+}
+
+template <int TYPE, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads)
+    mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
+                            int64_t lds, typename Element<TYPE>::type* __restrict__ out, int64_t ldo, int64_t rows,
+                            unsigned per_row, unsigned rows_per_block) {
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
+    const unsigned here = static_cast<unsigned>(min(static_cast<int64_t>(rows_per_block), rows - row0));
+    const unsigned total = here * per_row;
+    for (unsigned i = threadIdx.x; i < total; i += kThreads) {
+        const unsigned r = i / per_row, c = i - r * per_row;
+        const uint8_t* src = codes + (row0 + r) * ldc + static_cast<int64_t>(c) * (kChunk / 2);
+        uint32_t packed = 0;
+        if constexpr (ALIGNED) {
+            packed = *reinterpret_cast<const uint32_t*>(src);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) packed |= static_cast<uint32_t>(src[j]) << (8 * j);
+        }
+        const float scale = e8m0_value(scales[(row0 + r) * lds + c / 4]);
+        Chunk<TYPE> values;
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j)
+            values.v[j] = Element<TYPE>::from_float(grouped::e2m1_value(packed >> (4 * j)) * scale);
+        auto* dst = out + (row0 + r) * ldo + static_cast<int64_t>(c) * kChunk;
+        if constexpr (ALIGNED) {
+            *reinterpret_cast<Chunk<TYPE>*>(dst) = values;
+        } else {
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) dst[j] = values.v[j];
+        }
+    }
+}
+
+bool aligned(const void* p, int64_t stride_bytes, int to) {
+    return reinterpret_cast<uintptr_t>(p) % to == 0 && stride_bytes % to == 0;
+}
+
+// About four chunks a thread where there is enough for every SM, one where
+// there is not (a few rows: the call is as long as one thread's work).
+unsigned rows_per_block(int64_t rows, unsigned per_row) {
+    const int64_t chunks = rows * per_row;
+    const unsigned want = chunks > 8LL * kThreads * multiprocessor_count() ? 4 * kThreads : kThreads;
+    const unsigned fit = want / per_row;
+    return fit < 1 ? 1 : fit;
+}
+
+template <int TYPE>
+int quantize(const void* X, int64_t ldx, uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds, int64_t rows,
+             int K, cudaStream_t stream) {
+    using T = typename Element<TYPE>::type;
+    const unsigned per_row = K / kChunk, per_block = rows_per_block(rows, per_row);
+    const int64_t blocks = (rows + per_block - 1) / per_block;
+    if (blocks > 0x7fffffff) return KMCTS_EINVAL;
+    auto* x = static_cast<const T*>(X);
+    if (aligned(X, ldx * sizeof(T), 16) && aligned(codes, ldc, 4))
+        mxfp4_quantize_kernel<TYPE, true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+            x, ldx, codes, ldc, scales, lds, rows, per_row, per_block);
+    else
+        mxfp4_quantize_kernel<TYPE, false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+            x, ldx, codes, ldc, scales, lds, rows, per_row, per_block);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return cudaGetLastError() == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
+}
+
+template <int TYPE>
+int dequantize(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, void* out, int64_t ldo,
+               int64_t rows, int K, cudaStream_t stream) {
+    using T = typename Element<TYPE>::type;
+    const unsigned per_row = K / kChunk, per_block = rows_per_block(rows, per_row);
+    const int64_t blocks = (rows + per_block - 1) / per_block;
+    if (blocks > 0x7fffffff) return KMCTS_EINVAL;
+    auto* o = static_cast<T*>(out);
+    if (aligned(out, ldo * sizeof(T), 16) && aligned(codes, ldc, 4))
+        mxfp4_dequantize_kernel<TYPE, true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+            codes, ldc, scales, lds, o, ldo, rows, per_row, per_block);
+    else
+        mxfp4_dequantize_kernel<TYPE, false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+            codes, ldc, scales, lds, o, ldo, rows, per_row, per_block);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return cudaGetLastError() == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
+}
+
+}  // namespace
+}  // namespace kmcts
+
+using namespace kmcts;
+
+extern "C" {
+
+int kmcts_mxfp4_quantize(const void* X, int x_type, int64_t ldx, void* codes, int64_t ldc, void* scales, int64_t lds,
+                         int64_t rows, int K, void* stream) {
+    if (rows < 0 || K < 0 || K % 32 != 0) return KMCTS_EINVAL;
+    if (rows == 0 || K == 0) return KMCTS_OK;
+    if (!X || !codes || !scales || ldx < K || ldc < K / 2 || lds < K / 32) return KMCTS_EINVAL;
+    auto* c = static_cast<uint8_t*>(codes);
+    auto* s = static_cast<uint8_t*>(scales);
+    auto st = static_cast<cudaStream_t>(stream);
+    switch (x_type) {
+        case KMCTS_TYPE_BF16: return quantize<KMCTS_TYPE_BF16>(X, ldx, c, ldc, s, lds, rows, K, st);
+        case KMCTS_TYPE_FP16: return quantize<KMCTS_TYPE_FP16>(X, ldx, c, ldc, s, lds, rows, K, st);
+        case KMCTS_TYPE_FP32: return quantize<KMCTS_TYPE_FP32>(X, ldx, c, ldc, s, lds, rows, K, st);
+        default: return KMCTS_EINVAL;
+    }
+}
+
+int kmcts_mxfp4_dequantize(const void* codes, int64_t ldc, const void* scales, int64_t lds, void* out, int out_type,
+                           int64_t ldo, int64_t rows, int K, void* stream) {
+    if (rows < 0 || K < 0 || K % 32 != 0) return KMCTS_EINVAL;
+    if (rows == 0 || K == 0) return KMCTS_OK;
+    if (!codes || !scales || !out || ldo < K || ldc < K / 2 || lds < K / 32) return KMCTS_EINVAL;
+    auto* c = static_cast<const uint8_t*>(codes);
+    auto* s = static_cast<const uint8_t*>(scales);
+    auto st = static_cast<cudaStream_t>(stream);
+    switch (out_type) {
+        case KMCTS_TYPE_BF16: return dequantize<KMCTS_TYPE_BF16>(c, ldc, s, lds, out, ldo, rows, K, st);
+        case KMCTS_TYPE_FP16: return dequantize<KMCTS_TYPE_FP16>(c, ldc, s, lds, out, ldo, rows, K, st);
+        case KMCTS_TYPE_FP32: return dequantize<KMCTS_TYPE_FP32>(c, ldc, s, lds, out, ldo, rows, K, st);
+        default: return KMCTS_EINVAL;
+    }
+}
+
+}  // extern "C"

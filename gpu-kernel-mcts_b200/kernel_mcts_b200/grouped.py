@@ -1,0 +1,176 @@
+"""BF16 products grouped by expert, and their gradients.
+
+Rows are sorted by group: ``ends`` is an int32 tensor on the operands' device
+whose element ``e`` is one past the last row of group ``e`` (the row counts'
+running sum).  It is read on the device; no call waits for it.  Ends that
+decrease or exceed the rows only make groups empty or short.  Rows behind the
+last end belong to no group: results that the call allocates hold zeros there,
+an ``out`` that the caller gives is left as it was.
+
+The weight of group ``e`` is ``w[e]``: ``[N, K]`` for ``w_layout="col"``
+(``Y = X·W^T``, the column-major B of the dense GEMM) or ``[K, N]`` for
+``"row"`` (``Y = X·W``).  ``grouped_gemm(dy, w, ends, w_layout="row")`` on the
+weight of a ``"col"`` product is that product's input gradient,
+:func:`grouped_gemm_wgrad` its weights' gradient, and :func:`grouped_linear`
+ties the three together for autograd.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _launch, _native
+from .gemm import layout_code
+
+KERNELS = {"auto": _native.KERNEL_AUTO, "tcgen05": _native.KERNEL_TCGEN05, "simt": _native.KERNEL_SIMT}
+
+_BF16 = (torch.bfloat16,)
+
+
+def kernel_code(kernel: str, kernels: dict[str, int] = KERNELS) -> int:
+    try:
+        return kernels[kernel]
+    except KeyError as error:
+        raise ValueError(f"unknown kernel {kernel!r}; use one of {sorted(kernels)}") from error
+
+
+def grouped_gemm(
+    x: torch.Tensor,
+    w: torch.Tensor,
+    ends: torch.Tensor,
+    out: torch.Tensor | None = None,
+    *,
+    w_layout: str | int = "col",
+    kernel: str = "auto",
+    stream: torch.cuda.Stream | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Each row of ``x`` ``[rows, K]`` times its group's weight: ``[rows, N]``.
+
+    Rows may be strided; FP32 sums, one rounding.  Asynchronous on ``stream``
+    (the current one by default).  ``status`` is as for
+    :func:`kernel_mcts_b200.gemm.bf16_gemm`.
+    """
+    code = layout_code(w_layout)
+    device = x.device
+    _launch.check_tensor("x", x, 2, _BF16)
+    _launch.check_tensor("w", w, 3, _BF16, device)
+    groups = _launch.check_groups(ends, device)
+    rows, k = x.shape
+    n, kw = (w.shape[1], w.shape[2]) if code == _native.B_COL else (w.shape[2], w.shape[1])
+    if kw != k:
+        raise ValueError(f"inner dimensions differ: x has K={k}, w has K={kw}")
+    if w.shape[0] != groups:
+        raise ValueError(f"w holds {w.shape[0]} groups, ends {groups}")
+    ldx, ldw = _launch.row_stride("x", x, 0, 8), _launch.row_stride("w", w, 1, 8)
+    status_ptr = _launch.status_pointer(status, device)
+    kernel_id = kernel_code(kernel)
+    caller = _launch.caller_stream(device, stream)
+    with _launch.on_device(device, stream):
+        flags = 0
+        if out is None:
+            out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
+            _launch.share_result(out, caller)
+            flags = _native.GROUPED_ZERO_REST
+        else:
+            _launch.check_tensor("out", out, 2, _BF16, device)
+            if out.shape[0] != rows or out.shape[1] != n:
+                raise ValueError(f"out must have shape {(rows, n)}, got {tuple(out.shape)}")
+        rc = _native.load().kmcts_bf16_grouped_gemm(
+            x.data_ptr(), ldx, w.data_ptr(), w.stride(0) if groups > 1 else 0, ldw, code, out.data_ptr(),
+            _launch.row_stride("out", out, 0, 8), ends.data_ptr(), groups, rows, n, k, flags, kernel_id,
+            _launch.stream_handle(device, stream), status_ptr)
+    _native.check(rc, "kmcts_bf16_grouped_gemm")
+    return out
+
+
+def grouped_gemm_wgrad(
+    dy: torch.Tensor,
+    x: torch.Tensor,
+    ends: torch.Tensor,
+    out: torch.Tensor | None = None,
+    *,
+    dtype: torch.dtype | None = None,
+    accumulate: bool = False,
+    kernel: str = "auto",
+    stream: torch.cuda.Stream | None = None,
+    status: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``dy[rows of e]^T · x[rows of e]`` for every group: ``[groups, N, K]``.
+
+    The result is ``dtype`` (bfloat16 by default, or float32) or ``out``'s type.
+    ``accumulate`` adds to a float32 ``out``, as for a main gradient kept over
+    several micro-batches; an empty group then leaves its part as it was, and
+    is zeros otherwise.
+    """
+    device = dy.device
+    _launch.check_tensor("dy", dy, 2, _BF16)
+    _launch.check_tensor("x", x, 2, _BF16, device)
+    groups = _launch.check_groups(ends, device)
+    rows, n = dy.shape
+    k = x.shape[1]
+    if x.shape[0] != rows:
+        raise ValueError(f"dy has {rows} rows, x {x.shape[0]}")
+    lddy, ldx = _launch.row_stride("dy", dy, 0, 8), _launch.row_stride("x", x, 0, 8)
+    if dtype is None:
+        dtype = out.dtype if out is not None else torch.bfloat16
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"the gradient must be bfloat16 or float32, got {dtype}")
+    if accumulate and (out is None or dtype != torch.float32):
+        raise ValueError("accumulate needs a float32 out")
+    status_ptr = _launch.status_pointer(status, device)
+    kernel_id = kernel_code(kernel)
+    caller = _launch.caller_stream(device, stream)
+    with _launch.on_device(device, stream):
+        if out is None:
+            out = torch.empty((groups, n, k), dtype=dtype, device=device)
+            _launch.share_result(out, caller)
+        else:
+            _launch.check_tensor("out", out, 3, (dtype,), device)
+            if tuple(out.shape) != (groups, n, k):
+                raise ValueError(f"out must have shape {(groups, n, k)}, got {tuple(out.shape)}")
+        ldo = _launch.row_stride("out", out, 1, 8)
+        group_stride = out.stride(0) if groups > 1 else n * ldo
+        if groups > 1 and n > 0 and group_stride < (n - 1) * ldo + k:
+            raise ValueError("out has overlapping groups")
+        rc = _native.load().kmcts_bf16_grouped_wgrad(
+            dy.data_ptr(), lddy, x.data_ptr(), ldx, out.data_ptr(), group_stride, ldo,
+            _native.TYPE_FP32 if dtype == torch.float32 else _native.TYPE_BF16, int(accumulate), ends.data_ptr(), groups,
+            rows, n, k, kernel_id, _launch.stream_handle(device, stream), status_ptr)
+    _native.check(rc, "kmcts_bf16_grouped_wgrad")
+    return out
+
+
+def _strided_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` itself where the kernels can read it, else a contiguous copy (an
+    expanded gradient, as a sum's backward gives, has overlapping rows)."""
+    if t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+        return t
+    return t.contiguous()
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, ends):
+        ctx.save_for_backward(x, w, ends)
+        return grouped_gemm(x, w, ends)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, ends = ctx.saved_tensors
+        dy = _strided_rows(dy)
+        dx = grouped_gemm(dy, w, ends, w_layout="row") if ctx.needs_input_grad[0] else None
+        dw = grouped_gemm_wgrad(dy, x, ends) if ctx.needs_input_grad[1] else None
+        return dx, dw, None
+
+
+def grouped_linear(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    """Differentiable ``grouped_gemm(x, w, ends)`` for ``w`` of ``[groups, N, K]``.
+
+    The gradients of ``x`` and ``w`` are bfloat16; ``x``'s is zero in rows
+    behind the last group.  Once differentiable."""
+    return _GroupedLinear.apply(x, w, ends)
+
+
+__all__ = ["grouped_gemm", "grouped_gemm_wgrad", "grouped_linear"]

@@ -1,0 +1,332 @@
+"""Products grouped by expert on the GPU, against 64-bit products.
+
+Bars:
+* integer-valued inputs: every output bit (FP32 sums of small integers are
+  exact in any order, and one rounding follows);
+* N(0,1) inputs: products of two BF16 values are exact in FP32; a sum of L
+  terms in any order, each addition off by at most one FP32 step (2^-23, which
+  covers rounding and truncation), is off by at most g = L * 2^-23 * sum |a b|,
+  and the rounding to BF16 adds 2^-8 of the value: |y - ref| <= g + 2^-8 (|ref| + g).
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kernel_mcts_b200 import _native, grouped
+
+pytestmark = pytest.mark.gpu
+
+KERNELS = ["auto", "simt"]
+
+# Row counts by group: empty groups at both ends and between, single rows,
+# lengths around the tiles' edges.
+COUNTS = {
+    "one_row": [1],
+    "edges": [0, 1, 127, 0, 128, 129, 15, 16, 17, 0],
+    "long": [600, 0, 257, 3],
+    "empty": [0, 0, 0],
+}
+# (N, K): aligned and not, below and across tiles; 77 x 50 has no aligned row.
+SIZES = [(64, 64), (136, 200), (520, 328), (33, 264), (1, 8), (77, 50)]
+
+
+def ends_of(counts):
+    return torch.tensor(counts).cumsum(0).to(torch.int32).cuda()
+
+
+def integers(*shape, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return torch.randint(-2, 3, shape, generator=gen).to(torch.bfloat16).cuda()
+
+
+def normals(*shape, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=gen).to(torch.bfloat16).cuda()
+
+
+def forward64(x, w, counts, layout):
+    """The product and the product of magnitudes, zero behind the last group."""
+    n = w.shape[1] if layout == "col" else w.shape[2]
+    y, mag = (torch.zeros(x.shape[0], n, dtype=torch.float64, device=x.device) for _ in range(2))
+    lo = 0
+    for e, c in enumerate(counts):
+        m = w[e].double().T if layout == "col" else w[e].double()
+        y[lo:lo + c] = x[lo:lo + c].double() @ m
+        mag[lo:lo + c] = x[lo:lo + c].double().abs() @ m.abs()
+        lo += c
+    return y, mag
+
+
+def wgrad64(dy, x, counts):
+    out, mag, lo = [], [], 0
+    for c in counts:
+        d, v = dy[lo:lo + c].double().T, x[lo:lo + c].double()
+        out.append(d @ v)
+        mag.append(d.abs() @ v.abs())
+        lo += c
+    return torch.stack(out), torch.stack(mag)
+
+
+def within(y, ref, mag, length, half_step):
+    g = length * 2.0 ** -23 * mag
+    return bool(((y.double() - ref).abs() <= g + half_step * (ref.abs() + g)).all())
+
+
+def checked(call, *args, **kwargs):
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = call(*args, status=status, **kwargs)
+    torch.cuda.synchronize()
+    assert int(status.item()) == 0, f"device status {int(status.item()):#x}"
+    return out
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("layout", ["col", "row"])
+@pytest.mark.parametrize("counts", COUNTS.values(), ids=COUNTS)
+@pytest.mark.parametrize("n,k", SIZES)
+def test_forward_integers_bit_exact(cuda_device, kernel, layout, counts, n, k):
+    rows = sum(counts) + 5  # five rows behind the last group
+    x = integers(rows, k, seed=1)
+    w = integers(len(counts), *((n, k) if layout == "col" else (k, n)), seed=2)
+    y = checked(grouped.grouped_gemm, x, w, ends_of(counts), w_layout=layout, kernel=kernel)
+    ref, _ = forward64(x, w, counts, layout)
+    assert torch.equal(y, ref.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("layout", ["col", "row"])
+def test_forward_normals_within_bound(cuda_device, kernel, layout):
+    counts, n, k = [70, 0, 300, 1], 264, 1000
+    x = normals(sum(counts), k, seed=3)
+    w = normals(len(counts), *((n, k) if layout == "col" else (k, n)), seed=4)
+    y = checked(grouped.grouped_gemm, x, w, ends_of(counts), w_layout=layout, kernel=kernel)
+    ref, mag = forward64(x, w, counts, layout)
+    assert within(y, ref, mag, k, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_rows_of_other_groups_and_behind_the_last_do_not_enter(cuda_device, kernel):
+    """Infinities and NaN in one group's rows, in the weight of an empty group
+    and behind the last group stay there."""
+    counts, n, k = [20, 0, 37, 130, 6], 72, 96
+    x, w = integers(sum(counts) + 9, k, seed=5), integers(5, n, k, seed=6)
+    ref, _ = forward64(x, w, counts, "col")
+    x[20:57] = float("nan")  # group 2
+    x[-9:] = float("inf")
+    w[1] = float("nan")
+    y = checked(grouped.grouped_gemm, x, w, ends_of(counts), kernel=kernel)
+    keep = torch.ones(len(x), dtype=torch.bool)
+    keep[20:57] = False
+    assert torch.equal(y[keep], ref.to(torch.bfloat16)[keep])
+    assert y[20:57].isnan().all()
+    dy = integers(len(x), n, seed=7)
+    x[20:57] = integers(37, k, seed=8)
+    dy[-9:] = float("nan")
+    dw = checked(grouped.grouped_gemm_wgrad, dy, x, ends_of(counts), kernel=kernel)
+    assert torch.equal(dw, wgrad64(dy, x, counts)[0].to(torch.bfloat16))
+    # One group's NaN stays in its own gradient, whichever side of a boundary it is.
+    x[57:187] = float("inf")
+    dw = checked(grouped.grouped_gemm_wgrad, dy, x, ends_of(counts), kernel=kernel)
+    others = [0, 1, 2, 4]
+    assert torch.equal(dw[others], wgrad64(dy, x, counts)[0].to(torch.bfloat16)[others])
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_out_given_keeps_rows_behind_the_last_group(cuda_device, kernel):
+    counts, n, k = [3, 130], 40, 64
+    x, w = integers(140, k, seed=1), integers(2, n, k, seed=2)
+    wide = torch.full((140, n + 24), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = wide[:, 8:8 + n]
+    y = checked(grouped.grouped_gemm, x, w, ends_of(counts), out, kernel=kernel)
+    assert y.data_ptr() == out.data_ptr()
+    ref, _ = forward64(x, w, counts, "col")
+    assert torch.equal(out[:133], ref[:133].to(torch.bfloat16))
+    assert (out[133:] == 7).all() and (wide[:, :8] == 7).all() and (wide[:, 8 + n:] == 7).all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("layout", ["col", "row"])
+def test_strided_operands(cuda_device, kernel, layout):
+    """Rows with gaps, weights inside a larger tensor, and offsets that break
+    16-byte alignment (which the CUDA-core kernel then takes)."""
+    counts, n, k = [50, 2, 9], 48, 72
+    for offset in (8, 3):
+        x = integers(61, k + 16, seed=1)[:, offset:offset + k]
+        shape = (n, k) if layout == "col" else (k, n)
+        w = integers(3, shape[0] + 2, shape[1] + 24, seed=2)[:, 1:1 + shape[0], offset:offset + shape[1]]
+        y = checked(grouped.grouped_gemm, x, w, ends_of(counts), w_layout=layout,
+                    kernel=kernel if offset == 8 else "auto")
+        assert torch.equal(y, forward64(x, w, counts, layout)[0].to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_ends_out_of_order_or_range_are_clamped(cuda_device, kernel):
+    n, k = 64, 64
+    x, w = integers(200, k, seed=1), integers(5, n, k, seed=2)
+    ends = torch.tensor([50, 30, 2 ** 31 - 1, -7, 120], dtype=torch.int32, device="cuda")
+    y = checked(grouped.grouped_gemm, x, w, ends, kernel=kernel)
+    counts = [50, 0, 150, 0, 0]
+    assert torch.equal(y, forward64(x, w, counts, "col")[0].to(torch.bfloat16))
+    dw = checked(grouped.grouped_gemm_wgrad, x, x, ends, kernel=kernel)
+    assert torch.equal(dw, wgrad64(x, x, counts)[0].to(torch.bfloat16))
+
+
+def test_many_groups(cuda_device):
+    counts = [(7 * e) % 5 for e in range(1024)]
+    x, w = integers(sum(counts), 64, seed=1), integers(1024, 24, 64, seed=2)
+    y = checked(grouped.grouped_gemm, x, w, ends_of(counts))
+    assert torch.equal(y, forward64(x, w, counts, "col")[0].to(torch.bfloat16))
+    dw = checked(grouped.grouped_gemm_wgrad, y, x, ends_of(counts), dtype=torch.float32)
+    ref, mag = wgrad64(y, x, counts)
+    assert within(dw, ref, mag, 5, 2.0 ** -24)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("counts", COUNTS.values(), ids=COUNTS)
+@pytest.mark.parametrize("n,k", SIZES)
+def test_wgrad_integers_bit_exact(cuda_device, kernel, dtype, counts, n, k):
+    rows = sum(counts) + 5
+    dy, x = integers(rows, n, seed=1), integers(rows, k, seed=2)
+    dw = checked(grouped.grouped_gemm_wgrad, dy, x, ends_of(counts), dtype=dtype, kernel=kernel)
+    assert torch.equal(dw, wgrad64(dy, x, counts)[0].to(dtype))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_wgrad_normals_within_bound(cuda_device, kernel):
+    counts, n, k = [70, 0, 2000, 1], 136, 264
+    dy, x = normals(sum(counts), n, seed=3), normals(sum(counts), k, seed=4)
+    for dtype, half in ((torch.bfloat16, 2.0 ** -8), (torch.float32, 2.0 ** -24)):
+        dw = checked(grouped.grouped_gemm_wgrad, dy, x, ends_of(counts), dtype=dtype, kernel=kernel)
+        assert within(dw, *wgrad64(dy, x, counts), max(counts), half)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_wgrad_accumulates_into_fp32(cuda_device, kernel):
+    counts, n, k = [70, 0, 130, 1], 136, 200
+    dy, x = integers(sum(counts), n, seed=3), integers(sum(counts), k, seed=4)
+    wide = torch.full((4, n + 1, k + 12), 0.5, device="cuda")
+    out = wide[:, :n, 4:4 + k]
+    ref = wgrad64(dy, x, counts)[0]
+    for step in (1, 2):
+        dw = checked(grouped.grouped_gemm_wgrad, dy, x, ends_of(counts), out, accumulate=True, kernel=kernel)
+        assert dw.data_ptr() == out.data_ptr() and torch.equal(out, (0.5 + step * ref).float())
+    checked(grouped.grouped_gemm_wgrad, dy, x, ends_of(counts), out, kernel=kernel)
+    assert torch.equal(out, ref.float())
+    assert (wide[:, n:] == 0.5).all() and (wide[:, :, :4] == 0.5).all() and (wide[:, :, 4 + k:] == 0.5).all()
+
+
+def test_linear_gradients(cuda_device):
+    """Forward and both gradients through autograd, with an expanded output
+    gradient, against the formulas; and the derivative of a scalar against
+    differences of it."""
+    counts, n, k = [33, 0, 140, 7], 72, 104
+    x, w = integers(190, k, seed=1).requires_grad_(), integers(4, n, k, seed=2).requires_grad_()
+    ends = ends_of(counts)
+    y = grouped.grouped_linear(x, w, ends)
+    dy = integers(190, n, seed=3)
+    gx, gw = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    assert torch.equal(y, forward64(x.detach(), w.detach(), counts, "col")[0].to(torch.bfloat16))
+    assert torch.equal(gx, forward64(dy, w.detach(), counts, "row")[0].to(torch.bfloat16))
+    assert torch.equal(gw, wgrad64(dy, x.detach(), counts)[0].to(torch.bfloat16))
+    assert (gx[180:] == 0).all()
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))  # an expanded gradient
+    ones = torch.ones_like(dy)
+    assert torch.equal(gx, forward64(ones, w.detach(), counts, "row")[0].to(torch.bfloat16))
+    # The loss sum(y * dy) is linear in one entry of x or w, so a difference of
+    # two losses with integer inputs is its derivative exactly.
+    def loss(xv, wv):
+        return forward64(xv, wv, counts, "col")[0].mul(dy.double())[:180].sum()
+
+    gx, gw = torch.autograd.grad(grouped.grouped_linear(x, w, ends), (x, w), dy)
+    base = loss(x.detach(), w.detach())
+    for r, c in ((0, 0), (40, 103), (179, 5)):
+        moved = x.detach().clone()
+        moved[r, c] += 1
+        assert (loss(moved, w.detach()) - base).to(torch.bfloat16) == gx[r, c]
+    for e, i, j in ((0, 0, 0), (2, 71, 103), (3, 9, 50)):
+        moved = w.detach().clone()
+        moved[e, i, j] += 1
+        assert (loss(x.detach(), moved) - base).to(torch.bfloat16) == gw[e, i, j]
+
+
+def test_only_the_gradients_asked_for_are_computed(cuda_device):
+    x, w = integers(8, 16, seed=1), integers(1, 8, 16, seed=2).requires_grad_()
+    y = grouped.grouped_linear(x, w, ends_of([8]))
+    before = _native.launch_count()
+    y.backward(torch.ones_like(y))
+    assert _native.launch_count() == before + 1 and w.grad is not None
+
+
+def test_side_stream_and_graph_replay(cuda_device):
+    counts, n, k = [40, 3, 90], 128, 256
+    x, w = integers(sum(counts), k, seed=1), integers(3, n, k, seed=2)
+    ends, out = ends_of(counts), torch.empty(sum(counts), n, dtype=torch.bfloat16, device="cuda")
+    ref = forward64(x, w, counts, "col")[0].to(torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    y = grouped.grouped_gemm(x, w, ends, stream=side)
+    dw = grouped.grouped_gemm_wgrad(y, x, ends, stream=side, dtype=torch.float32)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, ref)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grouped.grouped_gemm(x, w, ends, out)
+        dw2 = grouped.grouped_gemm_wgrad(out, x, ends, dtype=torch.float32)
+    for counts in ([40, 3, 90], [0, 133, 0], [133, 0, 0]):
+        ends.copy_(ends_of(counts))  # the captured kernels read the ends as they are at replay
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, forward64(x, w, counts, "col")[0].to(torch.bfloat16))
+        ref, mag = wgrad64(out, x, counts)
+        assert within(dw2, ref, mag, 133, 2.0 ** -24)
+    assert within(dw, *wgrad64(y, x, [40, 3, 90]), 133, 2.0 ** -24)
+
+
+def test_repeated_calls_give_the_same_bits(cuda_device):
+    counts, n, k = [5, 0, 60, 19], 256, 2048
+    x, w, ends = normals(84, k, seed=1), normals(4, n, k, seed=2), ends_of(counts)
+    first = grouped.grouped_gemm(x, w, ends)
+    grads = grouped.grouped_gemm_wgrad(first, x, ends)
+    for _ in range(5):
+        assert torch.equal(grouped.grouped_gemm(x, w, ends), first)
+        assert torch.equal(grouped.grouped_gemm_wgrad(first, x, ends), grads)
+
+
+def test_refusals(cuda_device):
+    x, w, ends = integers(6, 16), integers(2, 8, 16), ends_of([2, 4])
+    for bad in (ends.long(), ends[:, None], torch.zeros(4, dtype=torch.int32, device="cuda")[::2]):
+        with pytest.raises(TypeError, match="ends"):
+            grouped.grouped_gemm(x, w, bad)
+    with pytest.raises(ValueError, match="ends must be on"):
+        grouped.grouped_gemm(x, w, ends.cpu())
+    with pytest.raises(ValueError, match="groups"):
+        grouped.grouped_gemm(x, w, ends[:1])
+    with pytest.raises(ValueError, match="groups"):
+        grouped.grouped_gemm(x, w[:0], ends[:0])
+    with pytest.raises(ValueError, match="inner dimensions"):
+        grouped.grouped_gemm(x, w, ends, w_layout="row")
+    with pytest.raises(ValueError, match="shape"):
+        grouped.grouped_gemm(x, w, ends, integers(6, 9))
+    with pytest.raises(ValueError, match="contiguous"):
+        grouped.grouped_gemm(integers(16, 6).T, w, ends)
+    with pytest.raises(ValueError, match="overlapping"):
+        grouped.grouped_gemm(x[:1].expand(6, 16), w, ends)
+    with pytest.raises(ValueError, match="kernel"):
+        grouped.grouped_gemm(x, w, ends, kernel="fast")
+    with pytest.raises(ValueError, match="status"):
+        grouped.grouped_gemm(x, w, ends, status=torch.zeros(1, device="cuda"))
+    with pytest.raises(ValueError, match="rows"):
+        grouped.grouped_gemm_wgrad(x[:5], x, ends)
+    with pytest.raises(ValueError, match="accumulate"):
+        grouped.grouped_gemm_wgrad(x, x, ends, accumulate=True)
+    with pytest.raises(TypeError, match="gradient"):
+        grouped.grouped_gemm_wgrad(x, x, ends, dtype=torch.float16)
+    with pytest.raises(ValueError, match="overlapping"):
+        grouped.grouped_gemm_wgrad(x, x, ends, torch.empty(16, 16, dtype=torch.bfloat16, device="cuda").expand(2, 16, 16))
+    # Shapes with nothing in them.
+    assert grouped.grouped_gemm(x[:0], w, ends).shape == (0, 8)
+    assert (grouped.grouped_gemm(x[:, :0], w[:, :, :0], ends) == 0).all()
+    assert (grouped.grouped_gemm_wgrad(x[:0], x[:0], ends) == 0).all()
