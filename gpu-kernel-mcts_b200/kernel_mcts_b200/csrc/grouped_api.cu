@@ -1,5 +1,37 @@
 // C entry points of the grouped products (declared in include/kmcts_grouped.h).
-#include "grouped_internal.h"
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "grouped_tiles.cuh"
+
+namespace kmcts {
+namespace grouped {
+
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle) {
+    static std::once_flag once;
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    std::call_once(once, [] {
+        void* entry = nullptr;
+        cudaDriverEntryPointQueryResult query;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &query) ==
+                cudaSuccess &&
+            query == cudaDriverEntryPointSuccess)
+            encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(entry);
+    });
+    const cuuint32_t steps[3] = {1, 1, 1};
+    cuuint64_t d[3], s[2];
+    cuuint32_t b[3];
+    for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
+    for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i];
+    return encode && encode(map, type, rank, const_cast<void*>(base), d, s, b, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+                         CUDA_SUCCESS;
+}
+
+}  // namespace grouped
+}  // namespace kmcts
 
 using namespace kmcts;
 using namespace kmcts::grouped;
@@ -12,8 +44,14 @@ bool bad_groups(const int32_t* ends, int groups, int rows, int n, int k) {
 
 int forward(const ForwardArgs& a, Operand kind, int kernel, cudaStream_t stream, int* status) {
     if (a.rows == 0 || a.n == 0) return KMCTS_OK;
-    (void)status;
-    if (kernel != KMCTS_KERNEL_AUTO && kernel != KMCTS_KERNEL_SIMT) return KMCTS_ENOTSUP;
+    if (kernel < KMCTS_KERNEL_AUTO || kernel > KMCTS_KERNEL_SIMT) return KMCTS_EINVAL;
+    // K = 0 (all zeros) has nothing to copy in; it is left to the CUDA cores.
+    if (kernel != KMCTS_KERNEL_SIMT && a.k > 0) {
+        if (!status) status = default_status_ptr();
+        if (!status) return KMCTS_EHANDLE;
+        const int rc = launch_forward_pair(a, kind, gemm::kDefaultWaitNs, stream, status);
+        if (rc != KMCTS_ENOTSUP || kernel == KMCTS_KERNEL_TCGEN05) return rc;
+    }
     return launch_forward_simt(a, kind, stream);
 }
 
@@ -52,9 +90,15 @@ int kmcts_bf16_grouped_wgrad(const void* dY, int64_t lddy, const void* X, int64_
     a.dw = dW, a.dw_stride = dw_stride, a.lddw = lddw;
     a.fp32 = dw_type == KMCTS_TYPE_FP32, a.accumulate = accumulate != 0;
     a.ends = ends, a.groups = groups, a.rows = rows, a.n = N, a.k = K;
-    (void)device_status;
-    if (kernel != KMCTS_KERNEL_AUTO && kernel != KMCTS_KERNEL_SIMT) return KMCTS_ENOTSUP;
-    return launch_wgrad_simt(a, static_cast<cudaStream_t>(stream));
+    if (kernel < KMCTS_KERNEL_AUTO || kernel > KMCTS_KERNEL_SIMT) return KMCTS_EINVAL;
+    auto s = static_cast<cudaStream_t>(stream);
+    if (kernel != KMCTS_KERNEL_SIMT && rows > 0) {
+        int* status = device_status ? device_status : default_status_ptr();
+        if (!status) return KMCTS_EHANDLE;
+        const int rc = launch_wgrad_pair(a, gemm::kDefaultWaitNs, s, status);
+        if (rc != KMCTS_ENOTSUP || kernel == KMCTS_KERNEL_TCGEN05) return rc;
+    }
+    return launch_wgrad_simt(a, s);
 }
 
 int kmcts_mxfp4_gemm(const void* A, int64_t lda, const void* A_scales, int64_t ldas, const void* B, int64_t b_stride,

@@ -1,0 +1,639 @@
+// Grouped products on CTA pairs: one tcgen05.mma.cta_group::2 computes 256
+// weight rows x up to 256 tokens (192 in MXFP4) across a cluster of two CTAs.
+//
+// The weight is the MMA's A and the tokens its B, the accumulator is the
+// output transposed: the ragged dimension is then the MMA's N, which an
+// instruction descriptor sets at run time in steps of 32, so a group of 70
+// tokens costs 96 columns, where tokens in the MMA's rows would cost 256.  A
+// group's tokens split evenly over its tiles.  The epilogue turns each chunk
+// round in shared memory and writes the valid tokens only.
+//
+// The weights' gradient (Kind::kWgrad) is the same pipeline with the output
+// gradient's columns as A, the input's as B, both MN-major, and the group's
+// rows as the contracted dimension.  Its last block of 64 rows may reach into
+// the next group: a warp of each CTA zeroes the foreign rows of the last
+// 16-row step in shared memory (both operands: 0 * inf is not 0), and the MMA
+// takes no further step.
+//
+// Roles per CTA: warp 0 TMA producer; warp 1 MMA (the pair's leader issues);
+// warps 2-5 epilogue; MXFP4 adds four warps that fetch scales, the gradient
+// one that zeroes tails.  Every CTA reads the groups' ends itself and walks
+// the tiles round-robin; nothing is decided on the host.  Every wait is
+// bounded.
+#include <mutex>
+
+#include "grouped_tiles.cuh"
+
+namespace kmcts {
+namespace grouped {
+namespace {
+
+constexpr int kAccCols = 256;      // TMEM columns from one accumulator to the next (MXFP4: 192)
+constexpr int kBaseThreads = 192;  // producer, MMA, four epilogue warps
+
+template <Kind KIND>
+struct Pair {
+    static constexpr bool kMx = KIND == Kind::kMxfp4;
+    static constexpr bool kGrad = KIND == Kind::kWgrad;
+    static constexpr bool kAMn = KIND == Kind::kRow || kGrad;  // A (and for the gradient B) MN-major
+    static constexpr int kThreads = kBaseThreads + (kMx ? 128 : kGrad ? 32 : 0);
+    static constexpr int kBK = kMx ? 256 : 64;                 // K elements of a stage: 128 bytes a row
+    static constexpr int kMaxWidth = kMx ? 192 : 256;
+    static constexpr int kABytes = 128 * 128;
+    static constexpr int kBBytes = kMaxWidth / 2 * 128;
+    // Scales of a stage: two words a row, of 128 weight rows and 256 tokens.
+    static constexpr int kScaleBytes = kMx ? 2 * 512 + 2 * 1024 : 0;
+    static constexpr int kStageBytes = kABytes + kBBytes + kScaleBytes;
+    // MXFP4: each stage's scales have TMEM columns of their own, 8 + 16.
+    static constexpr int kStages = kMx ? 5 : kGrad ? 5 : 6;
+    static constexpr int kScaleCols = 24;
+    static constexpr int kStagingBytes = kGrad ? 8192 : 2048;  // an epilogue warp's
+    static constexpr int kStagingOffset = kStages * kStageBytes;
+    static constexpr int kBarrierOffset = kStagingOffset + 4 * kStagingBytes;
+    static constexpr int kTableOffset = kBarrierOffset + 512;
+    static constexpr int smem_bytes(int groups) { return 1024 + kTableOffset + 8 * (groups + 1); }
+    static_assert(2 * kMaxWidth + (kMx ? kStages * kScaleCols : 0) <= 512, "TMEM columns");
+    static_assert(smem_bytes(KMCTS_MAX_GROUPS) <= kMaxSmem, "shared memory");
+};
+
+struct PairParams {
+    const int32_t* ends;
+    int groups, rows;
+    int n, k;           // the weight is n x k (MMA: n in A's rows; gradient: k in B's columns)
+    __nv_bfloat16* y;   // forward output
+    int64_t ldy;
+    bool vec;           // y rows take 16-byte stores
+    bool zero_rest;
+    bool fp32, accumulate;  // gradient
+    const uint8_t* x_scales;
+    int64_t ldxs;
+    const uint8_t* w_scales;
+    int64_t ws_stride, ldws;
+    bool vec_scales;
+    uint64_t limit_ns;
+    int* status;
+};
+
+// One tile: A rows from n0, B columns (tokens, or columns of the gradient)
+// from b0, `width` of them computed and `valid` stored, over `blocks` stages.
+struct Tile {
+    int e, n0, b0, width, valid, blocks;
+    int t0, tail;  // gradient: first contracted row, rows of the last block (0: full)
+};
+
+template <Kind KIND>
+__device__ __forceinline__ Tile tile_at(const GroupTable& table, const PairParams& p, int t) {
+    using L = Pair<KIND>;
+    Tile out = {};
+    out.e = group_of_tile(table, t);
+    const int in_group = t - table.tile[out.e];
+    const int first = table.row[out.e], rows = table.row[out.e + 1] - first;
+    if constexpr (L::kGrad) {
+        const int tiles_k = (p.k + L::kMaxWidth - 1) / L::kMaxWidth;
+        const TileCoord tc = tile_coord(in_group, (p.n + 255) / 256, tiles_k, 8);
+        out.n0 = tc.m_blk * 256;
+        out.b0 = tc.n_blk * L::kMaxWidth;
+        out.valid = min(L::kMaxWidth, p.k - out.b0);
+        out.blocks = (rows + L::kBK - 1) / L::kBK;
+        out.t0 = first;
+        out.tail = rows % L::kBK;
+    } else {
+        const int tiles_t = (rows + L::kMaxWidth - 1) / L::kMaxWidth;
+        const int step = round_up((rows + tiles_t - 1) / tiles_t, 32);
+        const TileCoord tc = tile_coord(in_group, tiles_t, (p.n + 255) / 256, 8);
+        out.n0 = tc.n_blk * 256;
+        out.b0 = first + tc.m_blk * step;
+        out.valid = min(step, first + rows - out.b0);
+        out.blocks = (p.k + L::kBK - 1) / L::kBK;
+    }
+    out.width = round_up(out.valid, 32);
+    return out;
+}
+
+struct Barriers {
+    uint64_t *full, *empty, *tmem_full, *tmem_empty, *drain, *landed, *fixed;
+};
+
+// A position in the ring of stages.
+template <int STAGES>
+struct Ring {
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ void next() {
+        if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
+template <Kind KIND>
+__global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
+    grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                        const __grid_constant__ CUtensorMap map_b_wide, const __grid_constant__ CUtensorMap map_c,
+                        const __grid_constant__ PairParams p) {
+    using L = Pair<KIND>;
+    constexpr int S = L::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarrierOffset);
+    const Barriers bar = {bars, bars + S, bars + 2 * S, bars + 2 * S + 2, bars + 2 * S + 4, bars + 2 * S + 5,
+                          bars + 3 * S + 5};
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * S + 5);
+    volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* no_abort = abort + 1;
+    int* table_smem = reinterpret_cast<int*>(smem + L::kTableOffset);
+    const GroupTable table = {table_smem, table_smem + p.groups + 1, p.groups};
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int rank = static_cast<int>(ptx::cluster_ctarank());
+    const bool leader = rank == 0;
+    const int first_tile = blockIdx.x / 2, tile_step = gridDim.x / 2;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            // MXFP4: besides the leader's byte count, four scale warps of each CTA.
+            ptx::mbar_init(&bar.full[s], L::kMx ? 9 : 1);
+            ptx::mbar_init(&bar.empty[s], 1);
+            ptx::mbar_init(&bar.landed[s], 1);
+            ptx::mbar_init(&bar.fixed[s], 2);
+        }
+        for (int a = 0; a < 2; ++a) {
+            ptx::mbar_init(&bar.tmem_full[a], 1);
+            ptx::mbar_init(&bar.tmem_empty[a], 8);
+        }
+        ptx::mbar_init(bar.drain, 1);
+        *abort = 0;
+        *no_abort = 0;
+        ptx::fence_mbarrier_init();
+        ptx::prefetch_tensormap(&map_a);
+        ptx::prefetch_tensormap(&map_b);
+        if constexpr (L::kGrad) ptx::prefetch_tensormap(&map_c);
+        if constexpr (!L::kGrad) ptx::prefetch_tensormap(&map_b_wide);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(tmem_slot, 512);
+        ptx::tmem_relinquish_pair();
+    }
+    if (warp == 2) {
+        const int tiles_a = (p.n + 255) / 256;
+        if constexpr (L::kGrad) {
+            const int per_group = tiles_a * ((p.k + L::kMaxWidth - 1) / L::kMaxWidth);
+            build_group_table(table, p.ends, p.rows, [&](int) { return per_group; });
+        } else {
+            build_group_table(table, p.ends, p.rows,
+                              [&](int rows) { return (rows + L::kMaxWidth - 1) / L::kMaxWidth * tiles_a; });
+        }
+    }
+    __syncwarp();
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync();  // the leader's barriers exist before the peer signals them
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int tiles = table.tiles();
+    constexpr int kAccStep = L::kMx ? 192 : kAccCols;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer
+        if (lane == 0) {
+            Ring<S> ring;
+            uint32_t issued = 0, issued_phase = 0;
+            bool ok = true;
+            for (int t = first_tile; t < tiles && ok; t += tile_step) {
+                const Tile w = tile_at<KIND>(table, p, t);
+                const int half = w.width / 2;
+                const int a0 = w.n0 + rank * 128, b0 = w.b0 + rank * half;
+                // MN-major operands come in boxes of 64 columns, tokens in
+                // boxes of 32 rows or, for a full half, one of 128 (96).
+                const int boxes = L::kGrad ? (half + 63) / 64 : (half + 31) / 32;
+                const bool wide = !L::kGrad && half == L::kMaxWidth / 2;
+                const uint32_t b_bytes = static_cast<uint32_t>(L::kGrad ? boxes * 8192 : wide ? half * 128 : boxes * 4096);
+                for (int kb = 0; kb < w.blocks; ++kb) {
+                    if (!ptx::mbar_wait(&bar.empty[ring.stage], ring.phase ^ 1u, p.limit_ns, abort)) {
+                        record_failure(p.status, abort, kRoleProducer);
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* sa = smem + ring.stage * L::kStageBytes;
+                    uint8_t* sb = sa + L::kABytes;
+                    uint32_t full = ptx::mapa_shared(ptx::smem_addr(&bar.full[ring.stage]), 0);
+                    if constexpr (L::kGrad) {
+                        // A ragged last block lands on this CTA's own barrier:
+                        // its tail is zeroed before the leader hears of it.
+                        if (w.tail != 0 && kb == w.blocks - 1) {
+                            ptx::mbar_arrive_expect_tx(&bar.landed[ring.stage], L::kABytes + b_bytes);
+                            if (leader) ptx::mbar_arrive(&bar.full[ring.stage]);
+                            full = ptx::mapa_shared(ptx::smem_addr(&bar.landed[ring.stage]), rank);
+                        } else if (leader) {
+                            ptx::mbar_arrive_expect_tx(&bar.full[ring.stage], 2 * (L::kABytes + b_bytes));
+                        }
+                        const int t0 = w.t0 + kb * 64;
+                        for (int i = 0; i < 2; ++i) ptx::tma_load_2d_pair(sa + i * 8192, &map_a, full, a0 + 64 * i, t0);
+                        for (int i = 0; i < boxes; ++i)
+                            ptx::tma_load_2d_pair(sb + i * 8192, &map_b, full, b0 + 64 * i, t0);
+                    } else {
+                        if (leader) ptx::mbar_arrive_expect_tx(&bar.full[ring.stage], 2 * (L::kABytes + b_bytes));
+                        const int k0 = kb * (L::kMx ? 128 : 64);  // MXFP4 maps count bytes
+                        if constexpr (L::kAMn) {
+                            for (int i = 0; i < 2; ++i)
+                                ptx::tma_load_3d_pair(sa + i * 8192, &map_a, full, a0 + 64 * i, k0, w.e);
+                        } else {
+                            ptx::tma_load_3d_pair(sa, &map_a, full, k0, a0, w.e);
+                        }
+                        if (wide) {
+                            ptx::tma_load_2d_pair(sb, &map_b_wide, full, k0, b0);
+                        } else {
+                            for (int i = 0; i < boxes; ++i)
+                                ptx::tma_load_2d_pair(sb + i * 4096, &map_b, full, k0, b0 + 32 * i);
+                        }
+                    }
+                    issued |= 1u << ring.stage;
+                    issued_phase = (issued_phase & ~(1u << ring.stage)) | (ring.phase << ring.stage);
+                    ring.next();
+                }
+            }
+            // The leader's full barriers count both CTAs' copies; none may be
+            // in flight when a CTA leaves.  (A ragged block's are waited for by
+            // the warp that zeroes its tail.)
+            for (int s = 0; s < S; ++s) {
+                if (leader && (issued & (1u << s)) &&
+                    !ptx::mbar_wait(&bar.full[s], (issued_phase >> s) & 1u, drain_limit(p.limit_ns), no_abort))
+                    record_failure(p.status, abort, kRoleDrain);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ----------------------------------------------------------------- MMA
+        if (lane == 0 && leader) {
+            Ring<S> ring;
+            uint32_t fixed_phase = 0;  // a bit per stage
+            int local = 0;
+            bool ok = true;
+            for (int t = first_tile; t < tiles && ok; t += tile_step) {
+                const Tile w = tile_at<KIND>(table, p, t);
+                if (w.blocks == 0) continue;
+                const int acc = local & 1;
+                if (!ptx::mbar_wait(&bar.tmem_empty[acc], ((local >> 1) & 1) ^ 1u, p.limit_ns, abort)) {
+                    record_failure(p.status, abort, kRoleMma);
+                    break;
+                }
+                ++local;
+                ptx::tc_fence_after();
+                const uint32_t d = tmem_base + acc * kAccStep;
+                const uint32_t idesc = L::kMx ? ptx::make_idesc_mxf4(256, w.width, 0)
+                                              : ptx::make_idesc_bf16_ab(256, w.width, L::kAMn, L::kGrad);
+                for (int kb = 0; kb < w.blocks; ++kb) {
+                    bool here = L::kMx ? ptx::mbar_wait_cluster(&bar.full[ring.stage], ring.phase, p.limit_ns, abort)
+                                       : ptx::mbar_wait(&bar.full[ring.stage], ring.phase, p.limit_ns, abort);
+                    int steps = 4;
+                    if constexpr (L::kGrad) {
+                        if (here && w.tail != 0 && kb == w.blocks - 1) {
+                            here = ptx::mbar_wait_cluster(&bar.fixed[ring.stage], (fixed_phase >> ring.stage) & 1u,
+                                                          p.limit_ns, abort);
+                            fixed_phase ^= 1u << ring.stage;
+                            steps = (w.tail + 15) / 16;
+                        }
+                    }
+                    if (!here) {
+                        record_failure(p.status, abort, kRoleMma);
+                        ok = false;
+                        break;
+                    }
+                    ptx::tc_fence_after();
+                    const uint32_t sa = ptx::smem_addr(smem + ring.stage * L::kStageBytes);
+                    const uint32_t sb = sa + L::kABytes;
+                    if constexpr (L::kMx) {
+                        // Scales of this stage: two words of 4 columns for the
+                        // weight rows, two of 8 for the tokens.
+                        const uint32_t ss = sb + L::kBBytes;
+                        const uint32_t ts = tmem_base + 2 * kAccStep + ring.stage * L::kScaleCols;
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            ptx::tmem_copy_scales<2>(ts + 4 * g, ptx::make_scale_desc(ss + 512 * g));
+                            ptx::tmem_copy_scales<2>(ts + 8 + 8 * g, ptx::make_scale_desc(ss + 1024 + 1024 * g));
+                            ptx::tmem_copy_scales<2>(ts + 12 + 8 * g, ptx::make_scale_desc(ss + 1536 + 1024 * g));
+                        }
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            const uint32_t id = static_cast<uint32_t>(kk % 2 * 2);
+                            ptx::umma_mxf4<2>(d, ptx::make_sw128_desc(sa + kk * 32, 16, 1024),
+                                              ptx::make_sw128_desc(sb + kk * 32, 16, 1024), idesc | id << 4 | id << 29,
+                                              ts + 4 * (kk / 2), ts + 8 + 8 * (kk / 2), (kb | kk) != 0);
+                        }
+                    } else {
+                        for (int kk = 0; kk < steps; ++kk) {
+                            const uint64_t adesc = L::kAMn ? ptx::make_sw128_desc(sa + kk * 2048, 8192, 1024)
+                                                           : ptx::make_sw128_desc(sa + kk * 32, 16, 1024);
+                            const uint64_t bdesc = L::kGrad ? ptx::make_sw128_desc(sb + kk * 2048, 8192, 1024)
+                                                            : ptx::make_sw128_desc(sb + kk * 32, 16, 1024);
+                            ptx::umma_bf16_pair(d, adesc, bdesc, idesc, (kb | kk) != 0);
+                        }
+                    }
+                    ptx::umma_commit_pair(&bar.empty[ring.stage], 3);
+                    ring.next();
+                }
+                if (ok) ptx::umma_commit_pair(&bar.tmem_full[acc], 3);
+            }
+            ptx::umma_commit_pair(bar.drain, 3);
+        }
+        __syncwarp();
+    } else if (warp < 6) {
+        // ------------------------------------------------------------ epilogue
+        const int quarter = warp % 4;
+        uint8_t* staging = smem + L::kStagingOffset + (warp - 2) * L::kStagingBytes;
+        int local = 0, stored = 0;
+        for (int t = first_tile; t < tiles; t += tile_step) {
+            const Tile w = tile_at<KIND>(table, p, t);
+            const bool computed = w.blocks != 0;
+            if (!computed && p.accumulate) continue;  // adds nothing
+            const int acc = local & 1;
+            if (computed) {
+                const bool ok = ptx::mbar_wait(&bar.tmem_full[acc], (local >> 1) & 1, p.limit_ns, abort);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    if (lane == 0) record_failure(p.status, abort, kRoleEpilogue);
+                    break;
+                }
+                ++local;
+                ptx::tc_fence_after();
+            }
+            const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                   static_cast<uint32_t>(acc * kAccStep);
+            const int n0 = w.n0 + rank * 128 + quarter * 32;
+#pragma unroll 1
+            for (int c = 0; c < w.width; c += 32) {
+                uint32_t r[32];
+                if (computed) {
+                    ptx::tmem_ld_32x32b_x32(lanes + c, r);
+                    ptx::tmem_wait_ld();
+                    if (c + 32 >= w.width) {
+                        ptx::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.tmem_empty[acc]), 0));
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) r[j] = 0;
+                }
+                if constexpr (!L::kGrad) {
+                    store_transposed(r, staging, p.y + static_cast<int64_t>(w.b0 + c) * p.ldy, p.ldy, w.valid - c, n0, p.n,
+                                     p.vec, lane);
+                } else {
+                    // Lanes are rows of the gradient: 32 rows x 32 columns go
+                    // through a swizzled buffer and out by TMA, which clips
+                    // them at the group's own edges.
+                    uint8_t* buf = staging + (stored & 1) * 4096;
+                    if (lane == 0) ptx::bulk_wait_group_read<1>();
+                    __syncwarp();
+                    if (p.fp32) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<uint4*>(buf + lane * 128 + (j ^ (lane & 7)) * 16) =
+                                make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                    } else {
+                        // 64-byte rows: 16-byte chunk XOR (row / 2) % 4.
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            *reinterpret_cast<uint4*>(buf + lane * 64 + (j ^ (lane >> 1 & 3)) * 16) =
+                                make_uint4(gemm::pack_bf16x2(r[8 * j], r[8 * j + 1]),
+                                           gemm::pack_bf16x2(r[8 * j + 2], r[8 * j + 3]),
+                                           gemm::pack_bf16x2(r[8 * j + 4], r[8 * j + 5]),
+                                           gemm::pack_bf16x2(r[8 * j + 6], r[8 * j + 7]));
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && n0 < p.n) {
+                        if (p.accumulate)
+                            ptx::tma_add_3d(&map_c, buf, w.b0 + c, n0, w.e);
+                        else
+                            ptx::tma_store_3d(&map_c, buf, w.b0 + c, n0, w.e);
+                        ptx::bulk_commit_group();
+                    }
+                    ++stored;
+                }
+            }
+        }
+        if constexpr (L::kGrad) {
+            if (lane == 0) ptx::bulk_wait_group_read<0>();  // shared memory outlives the stores' reads of it
+        }
+        __syncwarp();
+    } else if constexpr (L::kMx) {
+        // -------------------------------------------------------------- scales
+        // Thread i holds weight row i of this CTA's 128 and tokens i and
+        // i + 128 of the tile (both CTAs need every token's scales).  Four
+        // stages' loads are in flight at once; the ring's depth hides them.
+        const int i = threadIdx.x - kBaseThreads;
+        const int blocks32 = p.k / 32;
+        Ring<S> ring;
+        bool ok = true;
+        for (int t = first_tile; t < tiles && ok; t += tile_step) {
+            const Tile w = tile_at<KIND>(table, p, t);
+            const int n = w.n0 + rank * 128 + i;
+            const uint8_t* rows[3] = {
+                n < p.n ? p.w_scales + w.e * p.ws_stride + n * p.ldws : nullptr,
+                i < w.valid ? p.x_scales + (static_cast<int64_t>(w.b0) + i) * p.ldxs : nullptr,
+                i + 128 < w.valid ? p.x_scales + (static_cast<int64_t>(w.b0) + i + 128) * p.ldxs : nullptr};
+            for (int kb0 = 0; kb0 < w.blocks && ok; kb0 += 4) {
+                uint2 v[4][3];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int j = 0; j < 3; ++j)
+                        v[q][j] = rows[j] && kb0 + q < w.blocks
+                                      ? load_scales(rows[j], (kb0 + q) * 8, blocks32, p.vec_scales)
+                                      : make_uint2(0, 0);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (kb0 + q >= w.blocks || !ok) break;
+                    ok = __all_sync(0xffffffffu,
+                                    ptx::mbar_wait(&bar.empty[ring.stage], ring.phase ^ 1u, p.limit_ns, abort));
+                    if (!ok) {
+                        if (lane == 0) record_failure(p.status, abort, kRoleProducer);
+                        break;
+                    }
+                    uint8_t* ss = smem + ring.stage * L::kStageBytes + L::kABytes + L::kBBytes;
+                    *reinterpret_cast<uint32_t*>(ss + scale_word_offset(i)) = v[q][0].x;
+                    *reinterpret_cast<uint32_t*>(ss + 512 + scale_word_offset(i)) = v[q][0].y;
+#pragma unroll
+                    for (int j = 1; j < 3; ++j) {
+                        const uint32_t at = scale_word_offset(i + 128 * (j - 1));
+                        *reinterpret_cast<uint32_t*>(ss + 1024 + at) = v[q][j].x;
+                        *reinterpret_cast<uint32_t*>(ss + 2048 + at) = v[q][j].y;
+                    }
+                    ptx::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0)
+                        ptx::mbar_arrive_release_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.full[ring.stage]), 0));
+                    ring.next();
+                }
+            }
+        }
+        __syncwarp();
+    } else if constexpr (L::kGrad) {
+        // ---------------------------------------------------------------- tails
+        Ring<S> ring;
+        uint32_t landed_phase = 0;  // a bit per stage
+        for (int t = first_tile; t < tiles; t += tile_step) {
+            const Tile w = tile_at<KIND>(table, p, t);
+            for (int kb = 0; kb < w.blocks - 1; ++kb) ring.next();
+            if (w.blocks == 0) continue;
+            if (w.tail != 0) {
+                // Not cut short by a failure elsewhere: no copy may be in
+                // flight when this CTA leaves.
+                const bool ok = ptx::mbar_wait(&bar.landed[ring.stage], (landed_phase >> ring.stage) & 1u,
+                                               drain_limit(p.limit_ns), no_abort);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    if (lane == 0) record_failure(p.status, abort, kRoleProducer);
+                    break;
+                }
+                landed_phase ^= 1u << ring.stage;
+                // Rows tail .. next multiple of 16 of every box: 128 bytes each
+                // whatever the swizzle, which permutes within a row.
+                uint8_t* stage = smem + ring.stage * L::kStageBytes;
+                const int boxes = 2 + (w.width / 2 + 63) / 64;
+                const int first = w.tail, count = round_up(w.tail, 16) - w.tail;
+                for (int i = lane; i < boxes * count * 8; i += 32) {
+                    const int box = i / (count * 8), at = i % (count * 8);
+                    *reinterpret_cast<uint4*>(stage + box * 8192 + first * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+                }
+                ptx::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive_release_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.fixed[ring.stage]), 0));
+            }
+            ring.next();
+        }
+        __syncwarp();
+    }
+
+    if constexpr (!L::kGrad) {
+        if (p.zero_rest) zero_rest_rows(p.y, p.ldy, table.rows(), p.rows, p.n, blockIdx.x, gridDim.x);
+    }
+    __syncwarp();
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        // Every UMMA that touches this CTA's memory has completed (the
+        // leader's last commit arrives in both CTAs).
+        if (lane == 0 && !ptx::mbar_wait(bar.drain, 0, drain_limit(p.limit_ns), no_abort))
+            record_failure(p.status, abort, kRoleDrain);
+        __syncwarp();
+    }
+    ptx::cluster_sync();  // no CTA leaves while its peer may still signal it
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+constexpr int kMaxDevices = 64;
+
+template <Kind KIND>
+int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b_wide, const CUtensorMap& c,
+           const PairParams& p, int64_t tiles, cudaStream_t stream) {
+    using L = Pair<KIND>;
+    static std::mutex mu;
+    static bool configured[kMaxDevices] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) return KMCTS_EHANDLE;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!configured[device]) {
+            if (cudaFuncSetAttribute(grouped_pair_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     L::smem_bytes(KMCTS_MAX_GROUPS)) != cudaSuccess)
+                return KMCTS_EGEMM;
+            configured[device] = true;
+        }
+    }
+    const int64_t pairs = multiprocessor_count() / 2;
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    config.gridDim = dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)), 1, 1);
+    config.blockDim = dim3(L::kThreads, 1, 1);
+    config.dynamicSmemBytes = L::smem_bytes(p.groups);
+    config.stream = stream;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, grouped_pair_kernel<KIND>, a, b, b_wide, c, p);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return err == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
+}
+
+}  // namespace
+
+int launch_forward_pair(const ForwardArgs& f, Operand operand, uint64_t limit_ns, cudaStream_t stream, int* status) {
+    PairParams p = {};
+    p.ends = f.ends, p.groups = f.groups, p.rows = f.rows, p.n = f.n, p.k = f.k;
+    p.y = static_cast<__nv_bfloat16*>(f.y), p.ldy = f.ldy;
+    p.vec = reinterpret_cast<uintptr_t>(f.y) % 16 == 0 && f.ldy % 8 == 0;
+    p.zero_rest = f.zero_rest;
+    p.x_scales = f.x_scales, p.ldxs = f.ldxs;
+    p.w_scales = f.w_scales, p.ws_stride = f.ws_stride, p.ldws = f.ldws;
+    p.vec_scales = ((reinterpret_cast<uintptr_t>(f.x_scales) | reinterpret_cast<uintptr_t>(f.w_scales) | f.ldxs |
+                     f.ldws | f.ws_stride) &
+                    7) == 0;
+    p.limit_ns = limit_ns, p.status = status;
+    const bool mx = operand == Operand::kMxfp4, row = operand == Operand::kBf16Row;
+    const auto type = mx ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const uint64_t size = mx ? 1 : 2;
+    const uint64_t kd = mx ? f.k / 2 : f.k;  // contiguous elements of a row of K
+    const uint64_t n = f.n, groups = f.groups;
+    CUtensorMap a, b, b_wide;
+    {
+        const uint64_t group = f.groups > 1 ? f.w_stride : f.ldw * (row ? kd : n);
+        const uint64_t dims[3] = {row ? n : kd, row ? kd : n, groups};
+        const uint64_t strides[2] = {f.ldw * size, group * size};
+        const uint32_t box[3] = {mx ? 128u : 64u, row ? 64u : 128u, 1};
+        if (!encode_map(&a, type, 3, f.w, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return KMCTS_ENOTSUP;
+    }
+    const uint64_t dims[2] = {kd, static_cast<uint64_t>(f.rows)};
+    const uint64_t strides[1] = {f.ldx * size};
+    const uint32_t box[2] = {mx ? 128u : 64u, 32};
+    const uint32_t box_wide[2] = {box[0], mx ? 96u : 128u};
+    if (!encode_map(&b, type, 2, f.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_map(&b_wide, type, 2, f.x, dims, strides, box_wide, CU_TENSOR_MAP_SWIZZLE_128B))
+        return KMCTS_ENOTSUP;
+    const int64_t width = mx ? 192 : 256;
+    const int64_t tiles = (f.rows / width + f.groups) * ((f.n + 255) / 256);
+    if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;
+    switch (operand) {
+        case Operand::kBf16Col: return launch<Kind::kCol>(a, b, b_wide, a, p, tiles, stream);
+        case Operand::kBf16Row: return launch<Kind::kRow>(a, b, b_wide, a, p, tiles, stream);
+        case Operand::kMxfp4: return launch<Kind::kMxfp4>(a, b, b_wide, a, p, tiles, stream);
+    }
+    return KMCTS_EINVAL;
+}
+
+int launch_wgrad_pair(const WgradArgs& g, uint64_t limit_ns, cudaStream_t stream, int* status) {
+    PairParams p = {};
+    p.ends = g.ends, p.groups = g.groups, p.rows = g.rows, p.n = g.n, p.k = g.k;
+    p.fp32 = g.fp32, p.accumulate = g.accumulate;
+    p.limit_ns = limit_ns, p.status = status;
+    const uint64_t n = g.n, k = g.k, rows = g.rows;
+    CUtensorMap a, b, c;
+    auto encode_rows = [&](CUtensorMap* map, const void* base, uint64_t cols, int64_t ld) {
+        const uint64_t dims[2] = {cols, rows}, strides[1] = {static_cast<uint64_t>(ld) * 2};
+        const uint32_t box[2] = {64, 64};
+        return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    if (!encode_rows(&a, g.dy, n, g.lddy) || !encode_rows(&b, g.x, k, g.ldx)) return KMCTS_ENOTSUP;
+    {
+        const uint64_t size = g.fp32 ? 4 : 2;
+        const uint64_t group = g.groups > 1 ? g.dw_stride : g.lddw * n;
+        const uint64_t dims[3] = {k, n, static_cast<uint64_t>(g.groups)}, strides[2] = {g.lddw * size, group * size};
+        const uint32_t box[3] = {32, 32, 1};  // 128-byte rows in FP32, 64 in BF16
+        if (!encode_map(&c, g.fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, g.dw, dims,
+                        strides, box, g.fp32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+            return KMCTS_ENOTSUP;
+    }
+    const int64_t tiles = static_cast<int64_t>(g.groups) * ((g.n + 255) / 256) * ((g.k + 255) / 256);
+    if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;
+    return launch<Kind::kWgrad>(a, b, b, c, p, tiles, stream);
+}
+
+}  // namespace grouped
+}  // namespace kmcts

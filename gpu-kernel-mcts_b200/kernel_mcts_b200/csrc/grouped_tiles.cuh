@@ -1,0 +1,79 @@
+// What the tensor-core kernels of the grouped products share: operand kinds,
+// tensor maps, failure reporting and the transposed epilogue.
+#pragma once
+
+#include "gemm_common.cuh"
+#include "grouped_common.cuh"
+#include "ptx_grouped.cuh"
+
+namespace kmcts {
+namespace grouped {
+
+using gemm::drain_limit;
+using gemm::kDefaultWaitNs;
+using gemm::kMaxSmem;
+using gemm::kRoleDrain;
+using gemm::kRoleEpilogue;
+using gemm::kRoleMma;
+using gemm::kRoleProducer;
+using gemm::record_failure;
+using gemm::tile_coord;
+using gemm::TileCoord;
+
+// The products' operands, by how the MMA's A (the weight; for the weights'
+// gradient, the output gradient) lies in memory.
+enum class Kind { kCol, kRow, kMxfp4, kWgrad };
+
+__host__ __device__ constexpr int round_up(int v, int to) { return (v + to - 1) / to * to; }
+
+// One scale word (four blocks' bytes) of row `r` in the layout that
+// tcgen05.cp spreads over TMEM: 32 rows of 16 bytes, row r of 128 in byte
+// column 4 (r / 32) of row r % 32.
+__device__ __forceinline__ uint32_t scale_word_offset(int r) {
+    return static_cast<uint32_t>(r / 128 * 512 + r % 32 * 16 + r % 128 / 32 * 4);
+}
+
+// Eight consecutive scale bytes of a row starting at block `first` of `blocks`
+// (bytes past the end read as zero: any finite scale serves, the codes there
+// are zeros).  vec: the address is 8-byte aligned.
+__device__ __forceinline__ uint2 load_scales(const uint8_t* row, int first, int blocks, bool vec) {
+    if (first + 8 <= blocks && vec) return __ldg(reinterpret_cast<const uint2*>(row + first));
+    uint32_t w[2] = {0, 0};
+    for (int i = 0; i < 8 && first + i < blocks; ++i)
+        w[i / 4] |= static_cast<uint32_t>(__ldg(row + first + i)) << (8 * (i % 4));
+    return make_uint2(w[0], w[1]);
+}
+
+// Writes a 32-token chunk of an accumulator whose lanes are output columns:
+// lane l holds column col0 + l of tokens 0..31 in r[].  The values turn round
+// in a 32 x 64-byte staging buffer of the warp's own, so that four lanes write
+// 64 consecutive bytes of one token's row.
+__device__ __forceinline__ void store_transposed(const uint32_t (&r)[32], uint8_t* staging, __nv_bfloat16* y,
+                                                 int64_t ldy, int tokens, int col0, int n, bool vec, int lane) {
+    __syncwarp();  // the chunk before has been read
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+        *reinterpret_cast<__nv_bfloat16*>(staging + j * 64 + lane * 2) = __float2bfloat16_rn(__uint_as_float(r[j]));
+    __syncwarp();
+    const int col = col0 + lane % 4 * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int j = i * 8 + lane / 4;
+        if (j >= tokens || col >= n) continue;
+        __nv_bfloat16* dst = y + j * ldy + col;
+        const auto* src = reinterpret_cast<const __nv_bfloat16*>(staging + j * 64) + lane % 4 * 8;
+        if (vec && col + 8 <= n) {
+            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+        } else {
+            for (int b = 0; b < 8 && col + b < n; ++b) dst[b] = src[b];
+        }
+    }
+}
+
+// Host: a tensor map of `rank` dimensions (dims[0] innermost, strides in bytes
+// of dims 1..rank-1).  False where the driver refuses it (alignment).
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle);
+
+}  // namespace grouped
+}  // namespace kmcts
