@@ -69,7 +69,7 @@ struct PairParams {
     int64_t ldxs;
     const uint8_t* w_scales;
     int64_t ws_stride, ldws;
-    bool vec_scales;
+    int scale_align;  // bytes that every row of scales starts at a multiple of
     uint64_t limit_ns;
     int* status;
 };
@@ -129,8 +129,9 @@ struct Ring {
 
 template <Kind KIND>
 __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
-    grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                        const __grid_constant__ CUtensorMap map_b_wide, const __grid_constant__ CUtensorMap map_c,
+    grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b128,
+                        const __grid_constant__ CUtensorMap map_b64, const __grid_constant__ CUtensorMap map_b32,
+                        const __grid_constant__ CUtensorMap map_c,
                         const __grid_constant__ PairParams p) {
     using L = Pair<KIND>;
     constexpr int S = L::kStages;
@@ -167,9 +168,13 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
         *no_abort = 0;
         ptx::fence_mbarrier_init();
         ptx::prefetch_tensormap(&map_a);
-        ptx::prefetch_tensormap(&map_b);
-        if constexpr (L::kGrad) ptx::prefetch_tensormap(&map_c);
-        if constexpr (!L::kGrad) ptx::prefetch_tensormap(&map_b_wide);
+        ptx::prefetch_tensormap(&map_b64);
+        if constexpr (L::kGrad) {
+            ptx::prefetch_tensormap(&map_c);
+        } else {
+            ptx::prefetch_tensormap(&map_b128);
+            ptx::prefetch_tensormap(&map_b32);
+        }
     }
     if (warp == 1) {
         ptx::tmem_alloc_pair(tmem_slot, 512);
@@ -204,11 +209,13 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                 const Tile w = tile_at<KIND>(table, p, t);
                 const int half = w.width / 2;
                 const int a0 = w.n0 + rank * 128, b0 = w.b0 + rank * half;
-                // MN-major operands come in boxes of 64 columns, tokens in
-                // boxes of 32 rows or, for a full half, one of 128 (96).
-                const int boxes = L::kGrad ? (half + 63) / 64 : (half + 31) / 32;
-                const bool wide = !L::kGrad && half == L::kMaxWidth / 2;
-                const uint32_t b_bytes = static_cast<uint32_t>(L::kGrad ? boxes * 8192 : wide ? half * 128 : boxes * 4096);
+                // MN-major operands come in boxes of 64 columns, tokens in one
+                // box of the next size up (16 experts of 448 tokens, 4096 x
+                // 4096: several boxes of 32 rows took 238 us, one box @@ us).
+                const int boxes = (half + 63) / 64;
+                const CUtensorMap* mb = half > 64 ? &map_b128 : half > 32 ? &map_b64 : &map_b32;
+                const int box_rows = half > 64 ? L::kMaxWidth / 2 : half > 32 ? 64 : 32;
+                const uint32_t b_bytes = static_cast<uint32_t>(L::kGrad ? boxes * 8192 : box_rows * 128);
                 for (int kb = 0; kb < w.blocks; ++kb) {
                     if (!ptx::mbar_wait(&bar.empty[ring.stage], ring.phase ^ 1u, p.limit_ns, abort)) {
                         record_failure(p.status, abort, kRoleProducer);
@@ -231,7 +238,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                         const int t0 = w.t0 + kb * 64;
                         for (int i = 0; i < 2; ++i) ptx::tma_load_2d_pair(sa + i * 8192, &map_a, full, a0 + 64 * i, t0);
                         for (int i = 0; i < boxes; ++i)
-                            ptx::tma_load_2d_pair(sb + i * 8192, &map_b, full, b0 + 64 * i, t0);
+                            ptx::tma_load_2d_pair(sb + i * 8192, &map_b64, full, b0 + 64 * i, t0);
                     } else {
                         if (leader) ptx::mbar_arrive_expect_tx(&bar.full[ring.stage], 2 * (L::kABytes + b_bytes));
                         const int k0 = kb * (L::kMx ? 128 : 64);  // MXFP4 maps count bytes
@@ -241,12 +248,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                         } else {
                             ptx::tma_load_3d_pair(sa, &map_a, full, k0, a0, w.e);
                         }
-                        if (wide) {
-                            ptx::tma_load_2d_pair(sb, &map_b_wide, full, k0, b0);
-                        } else {
-                            for (int i = 0; i < boxes; ++i)
-                                ptx::tma_load_2d_pair(sb + i * 4096, &map_b, full, k0, b0 + 32 * i);
-                        }
+                        ptx::tma_load_2d_pair(sb, mb, full, k0, b0);
                     }
                     issued |= 1u << ring.stage;
                     issued_phase = (issued_phase & ~(1u << ring.stage)) | (ring.phase << ring.stage);
@@ -379,34 +381,41 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                     store_transposed(r, staging, p.y + static_cast<int64_t>(w.b0 + c) * p.ldy, p.ldy, w.valid - c, n0, p.n,
                                      p.vec, lane);
                 } else {
-                    // Lanes are rows of the gradient: 32 rows x 32 columns go
-                    // through a swizzled buffer and out by TMA, which clips
-                    // them at the group's own edges.
+                    // Lanes are rows of the gradient: 32 rows of 128 bytes (64
+                    // columns, 32 in FP32) go through a swizzled buffer and
+                    // out by TMA, which clips them at the group's own edges.
+                    // (64-byte rows of BF16 took twice as long as the MMAs at
+                    // 512 rows a group: 311 us for 16 x 4096 x 4096.)
+                    const bool second = !p.fp32 && (c & 32);
                     uint8_t* buf = staging + (stored & 1) * 4096;
-                    if (lane == 0) ptx::bulk_wait_group_read<1>();
-                    __syncwarp();
+                    if (!second) {
+                        if (lane == 0) ptx::bulk_wait_group_read<1>();
+                        __syncwarp();
+                    }
                     if (p.fp32) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
                             *reinterpret_cast<uint4*>(buf + lane * 128 + (j ^ (lane & 7)) * 16) =
                                 make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
                     } else {
-                        // 64-byte rows: 16-byte chunk XOR (row / 2) % 4.
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            *reinterpret_cast<uint4*>(buf + lane * 64 + (j ^ (lane >> 1 & 3)) * 16) =
+                            *reinterpret_cast<uint4*>(buf + lane * 128 + ((j + (second ? 4 : 0)) ^ (lane & 7)) * 16) =
                                 make_uint4(gemm::pack_bf16x2(r[8 * j], r[8 * j + 1]),
                                            gemm::pack_bf16x2(r[8 * j + 2], r[8 * j + 3]),
                                            gemm::pack_bf16x2(r[8 * j + 4], r[8 * j + 5]),
                                            gemm::pack_bf16x2(r[8 * j + 6], r[8 * j + 7]));
+                        // A last half chunk's other half lies past the row's end.
+                        if (!second && c + 32 < w.width) continue;
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0 && n0 < p.n) {
+                        const int col = w.b0 + (second ? c - 32 : c);
                         if (p.accumulate)
-                            ptx::tma_add_3d(&map_c, buf, w.b0 + c, n0, w.e);
+                            ptx::tma_add_3d(&map_c, buf, col, n0, w.e);
                         else
-                            ptx::tma_store_3d(&map_c, buf, w.b0 + c, n0, w.e);
+                            ptx::tma_store_3d(&map_c, buf, col, n0, w.e);
                         ptx::bulk_commit_group();
                     }
                     ++stored;
@@ -419,54 +428,75 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
         __syncwarp();
     } else if constexpr (L::kMx) {
         // -------------------------------------------------------------- scales
-        // Thread i holds weight row i of this CTA's 128 and tokens i and
-        // i + 128 of the tile (both CTAs need every token's scales).  Four
-        // stages' loads are in flight at once; the ring's depth hides them.
-        const int i = threadIdx.x - kBaseThreads;
+        // Thread i holds one of this CTA's 128 weight rows and two of the
+        // tile's tokens (both CTAs need every token's scales): rows l / 4 + 32
+        // (l % 4) + 8 warps for lane l, so that a warp's words lie side by side
+        // in shared memory.  Scales come four stages at a time, two 16-byte
+        // loads a row, and the next four stages' are under way while these are
+        // handed out.
+        const int i = (warp - 6) * 8 + lane / 4 + lane % 4 * 32;
         const int blocks32 = p.k / 32;
         Ring<S> ring;
         bool ok = true;
-        for (int t = first_tile; t < tiles && ok; t += tile_step) {
-            const Tile w = tile_at<KIND>(table, p, t);
+        int t = first_tile, kb0 = 0;
+        Tile w = {};
+        const uint8_t* rows[3] = {};
+        auto start_tile = [&] {
+            w = tile_at<KIND>(table, p, t);
             const int n = w.n0 + rank * 128 + i;
-            const uint8_t* rows[3] = {
-                n < p.n ? p.w_scales + w.e * p.ws_stride + n * p.ldws : nullptr,
-                i < w.valid ? p.x_scales + (static_cast<int64_t>(w.b0) + i) * p.ldxs : nullptr,
-                i + 128 < w.valid ? p.x_scales + (static_cast<int64_t>(w.b0) + i + 128) * p.ldxs : nullptr};
-            for (int kb0 = 0; kb0 < w.blocks && ok; kb0 += 4) {
-                uint2 v[4][3];
+            rows[0] = n < p.n ? p.w_scales + w.e * p.ws_stride + n * p.ldws : nullptr;
+            for (int j = 0; j < 2; ++j)
+                rows[1 + j] = i + 128 * j < w.valid ? p.x_scales + (static_cast<int64_t>(w.b0) + i + 128 * j) * p.ldxs : nullptr;
+        };
+        uint4 v[3][2], next[3][2];  // 32 bytes of each row: stages kb0 .. kb0 + 3
+        auto load = [&](uint4 (&to)[3][2]) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int j = 0; j < 3; ++j)
-                        v[q][j] = rows[j] && kb0 + q < w.blocks
-                                      ? load_scales(rows[j], (kb0 + q) * 8, blocks32, p.vec_scales)
-                                      : make_uint2(0, 0);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if (kb0 + q >= w.blocks || !ok) break;
-                    ok = __all_sync(0xffffffffu,
-                                    ptx::mbar_wait(&bar.empty[ring.stage], ring.phase ^ 1u, p.limit_ns, abort));
-                    if (!ok) {
-                        if (lane == 0) record_failure(p.status, abort, kRoleProducer);
-                        break;
-                    }
-                    uint8_t* ss = smem + ring.stage * L::kStageBytes + L::kABytes + L::kBBytes;
-                    *reinterpret_cast<uint32_t*>(ss + scale_word_offset(i)) = v[q][0].x;
-                    *reinterpret_cast<uint32_t*>(ss + 512 + scale_word_offset(i)) = v[q][0].y;
-#pragma unroll
-                    for (int j = 1; j < 3; ++j) {
-                        const uint32_t at = scale_word_offset(i + 128 * (j - 1));
-                        *reinterpret_cast<uint32_t*>(ss + 1024 + at) = v[q][j].x;
-                        *reinterpret_cast<uint32_t*>(ss + 2048 + at) = v[q][j].y;
-                    }
-                    ptx::fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0)
-                        ptx::mbar_arrive_release_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.full[ring.stage]), 0));
-                    ring.next();
-                }
+            for (int j = 0; j < 3; ++j) {
+                to[j][0] = to[j][1] = make_uint4(0, 0, 0, 0);
+                if (rows[j]) load_scales(rows[j], kb0 * 8, blocks32, p.scale_align, to[j]);
             }
+        };
+        if (t < tiles) {
+            start_tile();
+            load(v);
+        }
+        while (t < tiles && ok) {
+            const int here = min(4, w.blocks - kb0);
+            kb0 += 4;
+            if (kb0 >= w.blocks) {
+                kb0 = 0;
+                t += tile_step;
+                if (t < tiles) start_tile();
+            }
+            if (t < tiles) load(next);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (q >= here || !ok) break;
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bar.empty[ring.stage], ring.phase ^ 1u, p.limit_ns, abort));
+                if (!ok) {
+                    if (lane == 0) record_failure(p.status, abort, kRoleProducer);
+                    break;
+                }
+                uint8_t* ss = smem + ring.stage * L::kStageBytes + L::kABytes + L::kBBytes;
+#pragma unroll
+                for (int j = 0; j < 3; ++j) {
+                    const uint4 both = v[j][q / 2];
+                    const uint32_t at = j == 0 ? scale_word_offset(i) : 1024 + scale_word_offset(i + 128 * (j - 1));
+                    *reinterpret_cast<uint32_t*>(ss + at) = q % 2 ? both.z : both.x;
+                    *reinterpret_cast<uint32_t*>(ss + at + (j == 0 ? 512 : 1024)) = q % 2 ? both.w : both.y;
+                }
+                // The words are read by this CTA's own tensor core (through the
+                // async proxy, which the fence orders them for), so the
+                // arrival needs no release at cluster scope: that waits for
+                // the loads under way as well, and made a stage 1.2 us long
+                // (8192 x 8192 x 8192: 701 us).
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.full[ring.stage]), 0));
+                ring.next();
+            }
+#pragma unroll
+            for (int j = 0; j < 3; ++j) v[j][0] = next[j][0], v[j][1] = next[j][1];
         }
         __syncwarp();
     } else if constexpr (L::kGrad) {
@@ -496,10 +526,10 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                     const int box = i / (count * 8), at = i % (count * 8);
                     *reinterpret_cast<uint4*>(stage + box * 8192 + first * 128 + at * 16) = make_uint4(0, 0, 0, 0);
                 }
-                ptx::fence_proxy_async();
+                // Read by this CTA's own tensor core: see the scales' arrivals.
+                ptx::fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0)
-                    ptx::mbar_arrive_release_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.fixed[ring.stage]), 0));
+                if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.fixed[ring.stage]), 0));
             }
             ring.next();
         }
@@ -529,8 +559,8 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
 constexpr int kMaxDevices = 64;
 
 template <Kind KIND>
-int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b_wide, const CUtensorMap& c,
-           const PairParams& p, int64_t tiles, cudaStream_t stream) {
+int launch(const CUtensorMap& a, const CUtensorMap (&b)[3], const CUtensorMap& c, const PairParams& p, int64_t tiles,
+           cudaStream_t stream) {
     using L = Pair<KIND>;
     static std::mutex mu;
     static bool configured[kMaxDevices] = {};
@@ -558,7 +588,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b_wide
     config.stream = stream;
     config.attrs = attr;
     config.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&config, grouped_pair_kernel<KIND>, a, b, b_wide, c, p);
+    const cudaError_t err = cudaLaunchKernelEx(&config, grouped_pair_kernel<KIND>, a, b[0], b[1], b[2], c, p);
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return err == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
 }
@@ -573,16 +603,16 @@ int launch_forward_pair(const ForwardArgs& f, Operand operand, uint64_t limit_ns
     p.zero_rest = f.zero_rest;
     p.x_scales = f.x_scales, p.ldxs = f.ldxs;
     p.w_scales = f.w_scales, p.ws_stride = f.ws_stride, p.ldws = f.ldws;
-    p.vec_scales = ((reinterpret_cast<uintptr_t>(f.x_scales) | reinterpret_cast<uintptr_t>(f.w_scales) | f.ldxs |
-                     f.ldws | f.ws_stride) &
-                    7) == 0;
+    const uintptr_t starts = reinterpret_cast<uintptr_t>(f.x_scales) | reinterpret_cast<uintptr_t>(f.w_scales) |
+                             static_cast<uintptr_t>(f.ldxs | f.ldws | f.ws_stride);
+    p.scale_align = starts % 16 == 0 ? 16 : starts % 8 == 0 ? 8 : 1;
     p.limit_ns = limit_ns, p.status = status;
     const bool mx = operand == Operand::kMxfp4, row = operand == Operand::kBf16Row;
     const auto type = mx ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const uint64_t size = mx ? 1 : 2;
     const uint64_t kd = mx ? f.k / 2 : f.k;  // contiguous elements of a row of K
     const uint64_t n = f.n, groups = f.groups;
-    CUtensorMap a, b, b_wide;
+    CUtensorMap a, b[3];
     {
         const uint64_t group = f.groups > 1 ? f.w_stride : f.ldw * (row ? kd : n);
         const uint64_t dims[3] = {row ? n : kd, row ? kd : n, groups};
@@ -592,18 +622,18 @@ int launch_forward_pair(const ForwardArgs& f, Operand operand, uint64_t limit_ns
     }
     const uint64_t dims[2] = {kd, static_cast<uint64_t>(f.rows)};
     const uint64_t strides[1] = {f.ldx * size};
-    const uint32_t box[2] = {mx ? 128u : 64u, 32};
-    const uint32_t box_wide[2] = {box[0], mx ? 96u : 128u};
-    if (!encode_map(&b, type, 2, f.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_map(&b_wide, type, 2, f.x, dims, strides, box_wide, CU_TENSOR_MAP_SWIZZLE_128B))
-        return KMCTS_ENOTSUP;
+    const uint32_t box_rows[3] = {mx ? 96u : 128u, 64, 32};
+    for (int i = 0; i < 3; ++i) {
+        const uint32_t box[2] = {mx ? 128u : 64u, box_rows[i]};
+        if (!encode_map(&b[i], type, 2, f.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return KMCTS_ENOTSUP;
+    }
     const int64_t width = mx ? 192 : 256;
     const int64_t tiles = (f.rows / width + f.groups) * ((f.n + 255) / 256);
     if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;
     switch (operand) {
-        case Operand::kBf16Col: return launch<Kind::kCol>(a, b, b_wide, a, p, tiles, stream);
-        case Operand::kBf16Row: return launch<Kind::kRow>(a, b, b_wide, a, p, tiles, stream);
-        case Operand::kMxfp4: return launch<Kind::kMxfp4>(a, b, b_wide, a, p, tiles, stream);
+        case Operand::kBf16Col: return launch<Kind::kCol>(a, b, a, p, tiles, stream);
+        case Operand::kBf16Row: return launch<Kind::kRow>(a, b, a, p, tiles, stream);
+        case Operand::kMxfp4: return launch<Kind::kMxfp4>(a, b, a, p, tiles, stream);
     }
     return KMCTS_EINVAL;
 }
@@ -614,25 +644,26 @@ int launch_wgrad_pair(const WgradArgs& g, uint64_t limit_ns, cudaStream_t stream
     p.fp32 = g.fp32, p.accumulate = g.accumulate;
     p.limit_ns = limit_ns, p.status = status;
     const uint64_t n = g.n, k = g.k, rows = g.rows;
-    CUtensorMap a, b, c;
+    CUtensorMap a, b[3], c;
     auto encode_rows = [&](CUtensorMap* map, const void* base, uint64_t cols, int64_t ld) {
         const uint64_t dims[2] = {cols, rows}, strides[1] = {static_cast<uint64_t>(ld) * 2};
         const uint32_t box[2] = {64, 64};
         return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    if (!encode_rows(&a, g.dy, n, g.lddy) || !encode_rows(&b, g.x, k, g.ldx)) return KMCTS_ENOTSUP;
+    if (!encode_rows(&a, g.dy, n, g.lddy) || !encode_rows(&b[1], g.x, k, g.ldx)) return KMCTS_ENOTSUP;
+    b[0] = b[2] = b[1];  // not used
     {
         const uint64_t size = g.fp32 ? 4 : 2;
         const uint64_t group = g.groups > 1 ? g.dw_stride : g.lddw * n;
         const uint64_t dims[3] = {k, n, static_cast<uint64_t>(g.groups)}, strides[2] = {g.lddw * size, group * size};
-        const uint32_t box[3] = {32, 32, 1};  // 128-byte rows in FP32, 64 in BF16
+        const uint32_t box[3] = {g.fp32 ? 32u : 64u, 32, 1};
         if (!encode_map(&c, g.fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, g.dw, dims,
-                        strides, box, g.fp32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+                        strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
             return KMCTS_ENOTSUP;
     }
     const int64_t tiles = static_cast<int64_t>(g.groups) * ((g.n + 255) / 256) * ((g.k + 255) / 256);
     if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;
-    return launch<Kind::kWgrad>(a, b, b, c, p, tiles, stream);
+    return launch<Kind::kWgrad>(a, b, c, p, tiles, stream);
 }
 
 }  // namespace grouped

@@ -33,15 +33,40 @@ __device__ __forceinline__ uint32_t scale_word_offset(int r) {
     return static_cast<uint32_t>(r / 128 * 512 + r % 32 * 16 + r % 128 / 32 * 4);
 }
 
-// Eight consecutive scale bytes of a row starting at block `first` of `blocks`
+// 32 consecutive scale bytes of a row starting at block `first` of `blocks`
 // (bytes past the end read as zero: any finite scale serves, the codes there
-// are zeros).  vec: the address is 8-byte aligned.
-__device__ __forceinline__ uint2 load_scales(const uint8_t* row, int first, int blocks, bool vec) {
-    if (first + 8 <= blocks && vec) return __ldg(reinterpret_cast<const uint2*>(row + first));
-    uint32_t w[2] = {0, 0};
-    for (int i = 0; i < 8 && first + i < blocks; ++i)
-        w[i / 4] |= static_cast<uint32_t>(__ldg(row + first + i)) << (8 * (i % 4));
-    return make_uint2(w[0], w[1]);
+// are zeros).  The row starts at a multiple of `align` bytes, first is a
+// multiple of 32.
+__device__ __forceinline__ void load_scales(const uint8_t* row, int first, int blocks, int align, uint4 (&out)[2]) {
+    const uint8_t* src = row + first;
+    if (align == 16 && first + 32 <= blocks) {
+        out[0] = __ldg(reinterpret_cast<const uint4*>(src));
+        out[1] = __ldg(reinterpret_cast<const uint4*>(src + 16));
+        return;
+    }
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int left = blocks - first - 8 * i;
+        uint2 pair = make_uint2(0, 0);
+        if (align >= 8 && left >= 8) {
+            pair = __ldg(reinterpret_cast<const uint2*>(src + 8 * i));
+        } else {
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                if (b >= left) break;
+                const uint32_t byte = __ldg(src + 8 * i + b);
+                if (b < 4) {
+                    pair.x |= byte << (8 * b);
+                } else {
+                    pair.y |= byte << (8 * (b - 4));
+                }
+            }
+        }
+        w[2 * i] = pair.x, w[2 * i + 1] = pair.y;
+    }
+    out[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    out[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 // Writes a 32-token chunk of an accumulator whose lanes are output columns:

@@ -17,7 +17,11 @@ struct Element;
 template <>
 struct Element<KMCTS_TYPE_BF16> {
     using type = __nv_bfloat16;
-    static __device__ float to_float(type v) { return __bfloat162float(v); }
+    // A shift: the conversion instruction shares a unit with the 4-bit
+    // conversions, which it kept busy all the time (16384 x 8192: 115 us).
+    static __device__ float to_float(type v) {
+        return __uint_as_float(static_cast<uint32_t>(__bfloat16_as_ushort(v)) << 16);
+    }
     static __device__ type from_float(float v) { return __float2bfloat16_rn(v); }
 };
 template <>
@@ -48,8 +52,30 @@ __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
     return out;
 }
 
-// Rows of a block, so that a block has a few thousand elements whatever K is.
-// Chunk i of the block is chunk i % per_row of its row i / per_row.
+// Two E2M1 codes (a byte) to two FP16 values, exactly.
+__device__ __forceinline__ __half2 e2m1x2_values(uint32_t byte) {
+    uint32_t out;
+    asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(out) : "r"(byte));
+    return *reinterpret_cast<__half2*>(&out);
+}
+
+// A block of threads takes `rows_per_block` rows, so that it has a thousand
+// chunks or more whatever K is; chunk i of the block is chunk i % per_row of
+// its row i / per_row.  A thread loads four chunks before it works on the
+// first: one at a time left HBM half idle (16384 x 8192 from BF16 80 us).
+constexpr int kBatch = 4;
+
+struct Place {
+    int64_t row;
+    unsigned chunk;
+};
+
+__device__ __forceinline__ Place place_of(unsigned i, int64_t row0, unsigned per_row, unsigned rows_per_block) {
+    if (rows_per_block == 1) return {row0, i};
+    const unsigned r = i / per_row;
+    return {row0 + r, i - r * per_row};
+}
+
 template <int TYPE, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads)
     mxfp4_quantize_kernel(const typename Element<TYPE>::type* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
@@ -59,42 +85,55 @@ __global__ void __launch_bounds__(kThreads)
     const unsigned here = static_cast<unsigned>(min(static_cast<int64_t>(rows_per_block), rows - row0));
     const unsigned total = here * per_row;
     // per_row is a multiple of 4, so a block's four lanes take the loop together.
-    for (unsigned i = threadIdx.x; i < total; i += kThreads) {
-        const unsigned r = i / per_row, c = i - r * per_row;
-        const auto* src = x + (row0 + r) * ldx + static_cast<int64_t>(c) * kChunk;
-        float v[kChunk];
-        if constexpr (ALIGNED) {
-            const Chunk<TYPE> in = *reinterpret_cast<const Chunk<TYPE>*>(src);
+    for (unsigned first = threadIdx.x; first < total; first += kBatch * kThreads) {
+        Chunk<TYPE> in[kBatch];
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) v[j] = Element<TYPE>::to_float(in.v[j]);
-        } else {
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned i = first + b * kThreads;
+            if (i >= total) break;
+            const Place at = place_of(i, row0, per_row, rows_per_block);
+            const auto* src = x + at.row * ldx + static_cast<int64_t>(at.chunk) * kChunk;
+            if constexpr (ALIGNED) {
+                in[b] = *reinterpret_cast<const Chunk<TYPE>*>(src);
+            } else {
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) v[j] = Element<TYPE>::to_float(src[j]);
+                for (int j = 0; j < kChunk; ++j) in[b].v[j] = src[j];
+            }
         }
-        // Magnitudes compare as integers, and a NaN is larger than infinity.
-        uint32_t largest = 0;
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);
-        const uint32_t quad = 0xfu << (threadIdx.x & 28);
-        largest = max(largest, __shfl_xor_sync(quad, largest, 1));
-        largest = max(largest, __shfl_xor_sync(quad, largest, 2));
-        // floor(log2) is the exponent field less 127 (a subnormal's is 0, and
-        // below the smallest scale either way); E2M1's largest exponent is 2.
-        const uint32_t field = largest >> 23;
-        const uint32_t scale = field == 255 ? 255 : field > 2 ? field - 2 : 0;
-        // 1 / scale = 2^(127 - scale): exact, normal for every scale there is.
-        const float inverse = __uint_as_float(scale == 255 ? 0u : (254 - scale) << 23);
-        uint32_t packed = 0;
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned i = first + b * kThreads;
+            if (i >= total) break;
+            const Place at = place_of(i, row0, per_row, rows_per_block);
+            float v[kChunk];
 #pragma unroll
-        for (int j = 0; j < kChunk; j += 2) packed |= e2m1x2(v[j] * inverse, v[j + 1] * inverse) << (4 * j);
-        uint8_t* dst = codes + (row0 + r) * ldc + static_cast<int64_t>(c) * (kChunk / 2);
-        if constexpr (ALIGNED) {
-            *reinterpret_cast<uint32_t*>(dst) = packed;
-        } else {
+            for (int j = 0; j < kChunk; ++j) v[j] = Element<TYPE>::to_float(in[b].v[j]);
+            // Magnitudes compare as integers, and a NaN is larger than infinity.
+            uint32_t largest = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) dst[j] = static_cast<uint8_t>(packed >> (8 * j));
+            for (int j = 0; j < kChunk; ++j) largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);
+            const uint32_t quad = 0xfu << (threadIdx.x & 28);
+            largest = max(largest, __shfl_xor_sync(quad, largest, 1));
+            largest = max(largest, __shfl_xor_sync(quad, largest, 2));
+            // floor(log2) is the exponent field less 127 (a subnormal's is 0,
+            // and below the smallest scale either way); E2M1's largest
+            // exponent is 2.
+            const uint32_t field = largest >> 23;
+            const uint32_t scale = field == 255 ? 255 : field > 2 ? field - 2 : 0;
+            // 1 / scale = 2^(127 - scale): exact, normal for every scale there is.
+            const float inverse = __uint_as_float(scale == 255 ? 0u : (254 - scale) << 23);
+            uint32_t packed = 0;
+#pragma unroll
+            for (int j = 0; j < kChunk; j += 2) packed |= e2m1x2(v[j] * inverse, v[j + 1] * inverse) << (4 * j);
+            uint8_t* dst = codes + at.row * ldc + static_cast<int64_t>(at.chunk) * (kChunk / 2);
+            if constexpr (ALIGNED) {
+                *reinterpret_cast<uint32_t*>(dst) = packed;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dst[j] = static_cast<uint8_t>(packed >> (8 * j));
+            }
+            if ((at.chunk & 3) == 0) scales[at.row * lds + at.chunk / 4] = static_cast<uint8_t>(scale);
         }
-        if ((c & 3) == 0) scales[(row0 + r) * lds + c / 4] = static_cast<uint8_t>(scale);
     }
 }
 
@@ -106,27 +145,43 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
     const unsigned here = static_cast<unsigned>(min(static_cast<int64_t>(rows_per_block), rows - row0));
     const unsigned total = here * per_row;
-    for (unsigned i = threadIdx.x; i < total; i += kThreads) {
-        const unsigned r = i / per_row, c = i - r * per_row;
-        const uint8_t* src = codes + (row0 + r) * ldc + static_cast<int64_t>(c) * (kChunk / 2);
-        uint32_t packed = 0;
-        if constexpr (ALIGNED) {
-            packed = *reinterpret_cast<const uint32_t*>(src);
-        } else {
+    for (unsigned first = threadIdx.x; first < total; first += kBatch * kThreads) {
+        uint32_t packed[kBatch], scale[kBatch];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) packed |= static_cast<uint32_t>(src[j]) << (8 * j);
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned i = first + b * kThreads;
+            if (i >= total) break;
+            const Place at = place_of(i, row0, per_row, rows_per_block);
+            const uint8_t* src = codes + at.row * ldc + static_cast<int64_t>(at.chunk) * (kChunk / 2);
+            if constexpr (ALIGNED) {
+                packed[b] = *reinterpret_cast<const uint32_t*>(src);
+            } else {
+                packed[b] = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) packed[b] |= static_cast<uint32_t>(src[j]) << (8 * j);
+            }
+            scale[b] = scales[at.row * lds + at.chunk / 4];
         }
-        const float scale = e8m0_value(scales[(row0 + r) * lds + c / 4]);
-        Chunk<TYPE> values;
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j)
-            values.v[j] = Element<TYPE>::from_float(grouped::e2m1_value(packed >> (4 * j)) * scale);
-        auto* dst = out + (row0 + r) * ldo + static_cast<int64_t>(c) * kChunk;
-        if constexpr (ALIGNED) {
-            *reinterpret_cast<Chunk<TYPE>*>(dst) = values;
-        } else {
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned i = first + b * kThreads;
+            if (i >= total) break;
+            const Place at = place_of(i, row0, per_row, rows_per_block);
+            const float s = e8m0_value(scale[b]);
+            Chunk<TYPE> values;
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) dst[j] = values.v[j];
+            for (int j = 0; j < kChunk; j += 2) {
+                const float2 pair = __half22float2(e2m1x2_values(packed[b] >> (4 * j) & 0xff));
+                values.v[j] = Element<TYPE>::from_float(pair.x * s);
+                values.v[j + 1] = Element<TYPE>::from_float(pair.y * s);
+            }
+            auto* dst = out + at.row * ldo + static_cast<int64_t>(at.chunk) * kChunk;
+            if constexpr (ALIGNED) {
+                *reinterpret_cast<Chunk<TYPE>*>(dst) = values;
+            } else {
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) dst[j] = values.v[j];
+            }
         }
     }
 }
@@ -139,7 +194,7 @@ bool aligned(const void* p, int64_t stride_bytes, int to) {
 // there is not (a few rows: the call is as long as one thread's work).
 unsigned rows_per_block(int64_t rows, unsigned per_row) {
     const int64_t chunks = rows * per_row;
-    const unsigned want = chunks > 8LL * kThreads * multiprocessor_count() ? 4 * kThreads : kThreads;
+    const unsigned want = chunks > 8LL * kThreads * multiprocessor_count() ? kBatch * kThreads : kThreads;
     const unsigned fit = want / per_row;
     return fit < 1 ? 1 : fit;
 }

@@ -47,10 +47,6 @@ __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, const void* s
         : "memory");
 }
 
-// Makes this thread's generic-proxy shared-memory writes visible to async
-// proxy accesses that other CTAs of the cluster cause.
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
-
 // Each of the 32 rows of 16 bytes at `desc` goes to one TMEM lane of four
 // consecutive columns at `taddr`, repeated in all four lane quarters.
 template <int CTAS>
