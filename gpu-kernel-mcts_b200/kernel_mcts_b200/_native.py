@@ -63,6 +63,7 @@ INPUTS = {"uniform": 0, "randn": 1, "int": 2}
 
 # kmcts_grouped.h
 GROUPED_ZERO_REST = 1
+KERNEL_GROUPED_PAIR, KERNEL_GROUPED_SPLIT = 3, 4
 TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
 
 #: Every symbol the headers under include/ declare.

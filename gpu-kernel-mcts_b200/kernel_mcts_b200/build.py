@@ -33,7 +33,7 @@ COMMON_FLAGS = ["-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS, f"-I{INCLUDE}", f
 
 LIBRARY_SOURCES = ("gemm_tcgen05.cu", "gemm_tcgen05_pair.cu", "gemm_tcgen05_stream.cu", "gemm_simt.cu", "compare.cu",
                    "capi.cu", "ipc.cu", "selftest.cu", "workspace.cu", "host_gemm.cu")
-GROUPED_SOURCES = ("grouped_api.cu", "grouped_pair.cu", "grouped_simt.cu", "mxfp4_quantize.cu")
+GROUPED_SOURCES = ("grouped_api.cu", "grouped_pair.cu", "grouped_split.cu", "grouped_simt.cu", "mxfp4_quantize.cu")
 HEADERS = ("ptx_sm100.cuh", "gemm_common.cuh", "kmcts_internal.h")
 GROUPED_HEADERS = ("grouped_common.cuh", "grouped_internal.h", "grouped_tiles.cuh", "ptx_grouped.cuh")
 

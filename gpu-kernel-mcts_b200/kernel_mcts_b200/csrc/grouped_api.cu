@@ -1,6 +1,8 @@
 // C entry points of the grouped products (declared in include/kmcts_grouped.h).
 #include <cudaTypedefs.h>
 
+#include <cstdlib>
+
 #include <mutex>
 
 #include "grouped_tiles.cuh"
@@ -30,6 +32,34 @@ bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void
                          CUDA_SUCCESS;
 }
 
+bool encode_forward_maps(const ForwardArgs& f, Operand operand, CUtensorMap* w, CUtensorMap (&x)[3],
+                         const uint32_t (&box_rows)[3]) {
+    const bool mx = operand == Operand::kMxfp4, row = operand == Operand::kBf16Row;
+    const auto type = mx ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const uint64_t size = mx ? 1 : 2, n = f.n;
+    const uint64_t k = mx ? f.k / 2 : f.k;  // contiguous elements of a row
+    const uint32_t inner = mx ? 128 : 64;   // 128 bytes
+    {
+        const uint64_t group = f.groups > 1 ? f.w_stride : f.ldw * (row ? k : n);
+        const uint64_t dims[3] = {row ? n : k, row ? k : n, static_cast<uint64_t>(f.groups)};
+        const uint64_t strides[2] = {f.ldw * size, group * size};
+        const uint32_t box[3] = {inner, row ? 64u : 128u, 1};
+        if (!encode_map(w, type, 3, f.w, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return false;
+    }
+    const uint64_t dims[2] = {k, static_cast<uint64_t>(f.rows)}, strides[1] = {f.ldx * size};
+    for (int i = 0; i < 3; ++i) {
+        const uint32_t box[2] = {inner, box_rows[i]};
+        if (!encode_map(&x[i], type, 2, f.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return false;
+    }
+    return true;
+}
+
+int scale_alignment(const ForwardArgs& f) {
+    const uintptr_t starts = reinterpret_cast<uintptr_t>(f.x_scales) | reinterpret_cast<uintptr_t>(f.w_scales) |
+                             static_cast<uintptr_t>(f.ldxs | f.ldws | f.ws_stride);
+    return starts % 16 == 0 ? 16 : starts % 8 == 0 ? 8 : 1;
+}
+
 }  // namespace grouped
 }  // namespace kmcts
 
@@ -42,15 +72,26 @@ bool bad_groups(const int32_t* ends, int groups, int rows, int n, int k) {
     return rows < 0 || n < 0 || k < 0 || groups < 1 || groups > KMCTS_MAX_GROUPS || !ends;
 }
 
+// CTAs that share a tile of the few-rows kernel, or 0 for the pair kernel.
+int few_row_splits(const ForwardArgs& a) {
+    static const char* env = getenv("KSPLIT");
+    if (env) return atoi(env);
+    return a.rows <= 32LL * a.groups ? 4 : 0;
+}
+
 int forward(const ForwardArgs& a, Operand kind, int kernel, cudaStream_t stream, int* status) {
     if (a.rows == 0 || a.n == 0) return KMCTS_OK;
-    if (kernel < KMCTS_KERNEL_AUTO || kernel > KMCTS_KERNEL_SIMT) return KMCTS_EINVAL;
+    if (kernel < KMCTS_KERNEL_AUTO || kernel > KMCTS_KERNEL_GROUPED_SPLIT) return KMCTS_EINVAL;
     // K = 0 (all zeros) has nothing to copy in; it is left to the CUDA cores.
     if (kernel != KMCTS_KERNEL_SIMT && a.k > 0) {
         if (!status) status = default_status_ptr();
         if (!status) return KMCTS_EHANDLE;
-        const int rc = launch_forward_pair(a, kind, gemm::kDefaultWaitNs, stream, status);
-        if (rc != KMCTS_ENOTSUP || kernel == KMCTS_KERNEL_TCGEN05) return rc;
+        const int splits = kernel == KMCTS_KERNEL_GROUPED_PAIR   ? 0
+                           : kernel == KMCTS_KERNEL_GROUPED_SPLIT ? (few_row_splits(a) > 0 ? few_row_splits(a) : 2)
+                                                                  : few_row_splits(a);
+        const int rc = splits > 0 ? launch_forward_split(a, kind, splits, gemm::kDefaultWaitNs, stream, status)
+                                  : launch_forward_pair(a, kind, gemm::kDefaultWaitNs, stream, status);
+        if (rc != KMCTS_ENOTSUP || kernel != KMCTS_KERNEL_AUTO) return rc;
     }
     return launch_forward_simt(a, kind, stream);
 }
@@ -96,7 +137,7 @@ int kmcts_bf16_grouped_wgrad(const void* dY, int64_t lddy, const void* X, int64_
         int* status = device_status ? device_status : default_status_ptr();
         if (!status) return KMCTS_EHANDLE;
         const int rc = launch_wgrad_pair(a, gemm::kDefaultWaitNs, s, status);
-        if (rc != KMCTS_ENOTSUP || kernel == KMCTS_KERNEL_TCGEN05) return rc;
+        if (rc != KMCTS_ENOTSUP || kernel != KMCTS_KERNEL_AUTO) return rc;
     }
     return launch_wgrad_simt(a, s);
 }

@@ -47,6 +47,8 @@ enum class Operand { kBf16Col, kBf16Row, kMxfp4 };
 // The tensor-core launchers return KMCTS_ENOTSUP, having launched nothing, for
 // operands that TMA cannot address.
 int launch_forward_pair(const ForwardArgs& a, Operand kind, uint64_t limit_ns, cudaStream_t stream, int* status);
+int launch_forward_split(const ForwardArgs& a, Operand kind, int splits, uint64_t limit_ns, cudaStream_t stream,
+                         int* status);
 int launch_wgrad_pair(const WgradArgs& a, uint64_t limit_ns, cudaStream_t stream, int* status);
 
 int launch_forward_simt(const ForwardArgs& a, Operand kind, cudaStream_t stream);

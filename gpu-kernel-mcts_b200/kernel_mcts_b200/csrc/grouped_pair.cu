@@ -16,8 +16,8 @@
 // takes no further step.
 //
 // Roles per CTA: warp 0 TMA producer; warp 1 MMA (the pair's leader issues);
-// warps 2-5 epilogue; MXFP4 adds four warps that fetch scales, the gradient
-// one that zeroes tails.  Every CTA reads the groups' ends itself and walks
+// warps 2-5 epilogue; MXFP4 adds four warps that fetch scales and one that
+// issues their copies into TMEM, the gradient one that zeroes tails.  Every CTA reads the groups' ends itself and walks
 // the tiles round-robin; nothing is decided on the host.  Every wait is
 // bounded.
 #include <mutex>
@@ -36,7 +36,7 @@ struct Pair {
     static constexpr bool kMx = KIND == Kind::kMxfp4;
     static constexpr bool kGrad = KIND == Kind::kWgrad;
     static constexpr bool kAMn = KIND == Kind::kRow || kGrad;  // A (and for the gradient B) MN-major
-    static constexpr int kThreads = kBaseThreads + (kMx ? 128 : kGrad ? 32 : 0);
+    static constexpr int kThreads = kBaseThreads + (kMx ? 160 : kGrad ? 32 : 0);
     static constexpr int kBK = kMx ? 256 : 64;                 // K elements of a stage: 128 bytes a row
     static constexpr int kMaxWidth = kMx ? 192 : 256;
     static constexpr int kABytes = 128 * 128;
@@ -111,20 +111,11 @@ __device__ __forceinline__ Tile tile_at(const GroupTable& table, const PairParam
 }
 
 struct Barriers {
-    uint64_t *full, *empty, *tmem_full, *tmem_empty, *drain, *landed, *fixed;
-};
-
-// A position in the ring of stages.
-template <int STAGES>
-struct Ring {
-    int stage = 0;
-    uint32_t phase = 0;
-    __device__ void next() {
-        if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-        }
-    }
+    uint64_t *full, *empty;            // a stage's operands are here; its MMAs are done
+    uint64_t *tmem_full, *tmem_empty;  // an accumulator is complete; it has been read
+    uint64_t* drain;                   // every MMA is done
+    uint64_t *landed, *fixed;          // gradient: a ragged block is here; its tail is zeroed
+    uint64_t *copied, *copies_done;    // MXFP4: a stage's scales are in TMEM; all of them are
 };
 
 template <Kind KIND>
@@ -138,9 +129,16 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarrierOffset);
-    const Barriers bar = {bars, bars + S, bars + 2 * S, bars + 2 * S + 2, bars + 2 * S + 4, bars + 2 * S + 5,
-                          bars + 3 * S + 5};
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * S + 5);
+    const Barriers bar = {bars,
+                          bars + S,
+                          bars + 2 * S,
+                          bars + 2 * S + 2,
+                          bars + 2 * S + 4,
+                          bars + 2 * S + 5,
+                          bars + 3 * S + 5,
+                          bars + 4 * S + 5,
+                          bars + 5 * S + 5};
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 5 * S + 6);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* no_abort = abort + 1;
     int* table_smem = reinterpret_cast<int*>(smem + L::kTableOffset);
@@ -158,12 +156,14 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
             ptx::mbar_init(&bar.empty[s], 1);
             ptx::mbar_init(&bar.landed[s], 1);
             ptx::mbar_init(&bar.fixed[s], 2);
+            ptx::mbar_init(&bar.copied[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
             ptx::mbar_init(&bar.tmem_full[a], 1);
             ptx::mbar_init(&bar.tmem_empty[a], 8);
         }
         ptx::mbar_init(bar.drain, 1);
+        ptx::mbar_init(bar.copies_done, 1);
         *abort = 0;
         *no_abort = 0;
         ptx::fence_mbarrier_init();
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                 const int a0 = w.n0 + rank * 128, b0 = w.b0 + rank * half;
                 // MN-major operands come in boxes of 64 columns, tokens in one
                 // box of the next size up (16 experts of 448 tokens, 4096 x
-                // 4096: several boxes of 32 rows took 238 us, one box @@ us).
+                // 4096: several boxes of 32 rows took 238 us, one box 205).
                 const int boxes = (half + 63) / 64;
                 const CUtensorMap* mb = half > 64 ? &map_b128 : half > 32 ? &map_b64 : &map_b32;
                 const int box_rows = half > 64 ? L::kMaxWidth / 2 : half > 32 ? 64 : 32;
@@ -286,8 +286,9 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                 const uint32_t idesc = L::kMx ? ptx::make_idesc_mxf4(256, w.width, 0)
                                               : ptx::make_idesc_bf16_ab(256, w.width, L::kAMn, L::kGrad);
                 for (int kb = 0; kb < w.blocks; ++kb) {
-                    bool here = L::kMx ? ptx::mbar_wait_cluster(&bar.full[ring.stage], ring.phase, p.limit_ns, abort)
-                                       : ptx::mbar_wait(&bar.full[ring.stage], ring.phase, p.limit_ns, abort);
+                    // MXFP4: the scales' copy has waited for the whole stage.
+                    bool here = ptx::mbar_wait(L::kMx ? &bar.copied[ring.stage] : &bar.full[ring.stage], ring.phase,
+                                               p.limit_ns, abort);
                     int steps = 4;
                     if constexpr (L::kGrad) {
                         if (here && w.tail != 0 && kb == w.blocks - 1) {
@@ -306,16 +307,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                     const uint32_t sa = ptx::smem_addr(smem + ring.stage * L::kStageBytes);
                     const uint32_t sb = sa + L::kABytes;
                     if constexpr (L::kMx) {
-                        // Scales of this stage: two words of 4 columns for the
-                        // weight rows, two of 8 for the tokens.
-                        const uint32_t ss = sb + L::kBBytes;
                         const uint32_t ts = tmem_base + 2 * kAccStep + ring.stage * L::kScaleCols;
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            ptx::tmem_copy_scales<2>(ts + 4 * g, ptx::make_scale_desc(ss + 512 * g));
-                            ptx::tmem_copy_scales<2>(ts + 8 + 8 * g, ptx::make_scale_desc(ss + 1024 + 1024 * g));
-                            ptx::tmem_copy_scales<2>(ts + 12 + 8 * g, ptx::make_scale_desc(ss + 1536 + 1024 * g));
-                        }
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
                             const uint32_t id = static_cast<uint32_t>(kk % 2 * 2);
@@ -424,6 +416,43 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
         }
         if constexpr (L::kGrad) {
             if (lane == 0) ptx::bulk_wait_group_read<0>();  // shared memory outlives the stores' reads of it
+        }
+        __syncwarp();
+    } else if (L::kMx && warp == 10) {
+        // ------------------------------------------------- scales into TMEM
+        // Per stage two words of 4 columns for the weight rows, two of 8 for
+        // the tokens.  Its own thread issues the copies and a commit tells the
+        // MMA's: issued by the MMA's thread itself they ran between its MMAs,
+        // 50 cycles each (8192 x 8192 x 8192: 360 us, 277 apart).
+        if (lane == 0 && leader) {
+            Ring<S> ring;
+            bool ok = true;
+            for (int t = first_tile; t < tiles && ok; t += tile_step) {
+                const Tile w = tile_at<KIND>(table, p, t);
+                for (int kb = 0; kb < w.blocks; ++kb) {
+                    if (!ptx::mbar_wait_cluster(&bar.full[ring.stage], ring.phase, p.limit_ns, abort)) {
+                        record_failure(p.status, abort, kRoleMma);
+                        ok = false;
+                        break;
+                    }
+                    ptx::tc_fence_after();
+                    const uint32_t ss =
+                        ptx::smem_addr(smem + ring.stage * L::kStageBytes) + L::kABytes + L::kBBytes;
+                    const uint32_t ts = tmem_base + 2 * kAccStep + ring.stage * L::kScaleCols;
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        ptx::tmem_copy_scales<2>(ts + 4 * g, ptx::make_scale_desc(ss + 512 * g));
+                        ptx::tmem_copy_scales<2>(ts + 8 + 8 * g, ptx::make_scale_desc(ss + 1024 + 1024 * g));
+                        ptx::tmem_copy_scales<2>(ts + 12 + 8 * g, ptx::make_scale_desc(ss + 1536 + 1024 * g));
+                    }
+                    ptx::umma_commit_pair(&bar.copied[ring.stage], 1);
+                    ring.next();
+                }
+            }
+            // No copy is under way when the CTAs leave, whatever the MMAs did.
+            ptx::umma_commit_pair(bar.copies_done, 1);
+            if (!ptx::mbar_wait(bar.copies_done, 0, drain_limit(p.limit_ns), no_abort))
+                record_failure(p.status, abort, kRoleDrain);
         }
         __syncwarp();
     } else if constexpr (L::kMx) {
@@ -603,30 +632,12 @@ int launch_forward_pair(const ForwardArgs& f, Operand operand, uint64_t limit_ns
     p.zero_rest = f.zero_rest;
     p.x_scales = f.x_scales, p.ldxs = f.ldxs;
     p.w_scales = f.w_scales, p.ws_stride = f.ws_stride, p.ldws = f.ldws;
-    const uintptr_t starts = reinterpret_cast<uintptr_t>(f.x_scales) | reinterpret_cast<uintptr_t>(f.w_scales) |
-                             static_cast<uintptr_t>(f.ldxs | f.ldws | f.ws_stride);
-    p.scale_align = starts % 16 == 0 ? 16 : starts % 8 == 0 ? 8 : 1;
+    p.scale_align = scale_alignment(f);
     p.limit_ns = limit_ns, p.status = status;
-    const bool mx = operand == Operand::kMxfp4, row = operand == Operand::kBf16Row;
-    const auto type = mx ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    const uint64_t size = mx ? 1 : 2;
-    const uint64_t kd = mx ? f.k / 2 : f.k;  // contiguous elements of a row of K
-    const uint64_t n = f.n, groups = f.groups;
-    CUtensorMap a, b[3];
-    {
-        const uint64_t group = f.groups > 1 ? f.w_stride : f.ldw * (row ? kd : n);
-        const uint64_t dims[3] = {row ? n : kd, row ? kd : n, groups};
-        const uint64_t strides[2] = {f.ldw * size, group * size};
-        const uint32_t box[3] = {mx ? 128u : 64u, row ? 64u : 128u, 1};
-        if (!encode_map(&a, type, 3, f.w, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return KMCTS_ENOTSUP;
-    }
-    const uint64_t dims[2] = {kd, static_cast<uint64_t>(f.rows)};
-    const uint64_t strides[1] = {f.ldx * size};
+    const bool mx = operand == Operand::kMxfp4;
     const uint32_t box_rows[3] = {mx ? 96u : 128u, 64, 32};
-    for (int i = 0; i < 3; ++i) {
-        const uint32_t box[2] = {mx ? 128u : 64u, box_rows[i]};
-        if (!encode_map(&b[i], type, 2, f.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return KMCTS_ENOTSUP;
-    }
+    CUtensorMap a, b[3];
+    if (!encode_forward_maps(f, operand, &a, b, box_rows)) return KMCTS_ENOTSUP;
     const int64_t width = mx ? 192 : 256;
     const int64_t tiles = (f.rows / width + f.groups) * ((f.n + 255) / 256);
     if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;

@@ -26,6 +26,19 @@ enum class Kind { kCol, kRow, kMxfp4, kWgrad };
 
 __host__ __device__ constexpr int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
+// A position in a ring of stages.
+template <int STAGES>
+struct Ring {
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ void next() {
+        if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
 // One scale word (four blocks' bytes) of row `r` in the layout that
 // tcgen05.cp spreads over TMEM: 32 rows of 16 bytes, row r of 128 in byte
 // column 4 (r / 32) of row r % 32.
@@ -99,6 +112,15 @@ __device__ __forceinline__ void store_transposed(const uint32_t (&r)[32], uint8_
 // of dims 1..rank-1).  False where the driver refuses it (alignment).
 bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
                 const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle);
+
+// Host: the weight's map (128 rows of 128 bytes, or for kBf16Row two boxes of
+// 64 x 64) and three of the tokens', by rows of a box.
+bool encode_forward_maps(const ForwardArgs& f, Operand operand, CUtensorMap* w, CUtensorMap (&x)[3],
+                         const uint32_t (&box_rows)[3]);
+
+// Host: the largest of 16, 8 and 1 bytes that every row of scales starts at a
+// multiple of.
+int scale_alignment(const ForwardArgs& f);
 
 }  // namespace grouped
 }  // namespace kmcts

@@ -6,7 +6,7 @@
 // needs no other lane and whose addresses cost one calculation, half a block
 // in FP32.  16384 x 8192 on B200: 54 us from BF16 (6.3 TB/s), against 110 us
 // with 8 elements a thread (three times the instructions); from FP32 a whole
-// block a thread took 128 us (128 bytes a lane outrun L1), half a block @@ us.
+// block a thread took 128 us (128 bytes a lane outrun L1), half a block 91 us.
 // Restoring, a thread writes 8 elements at a time, four times (58 us).
 #include "grouped_common.cuh"
 

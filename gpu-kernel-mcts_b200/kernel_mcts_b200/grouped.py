@@ -22,7 +22,9 @@ import torch
 from . import _launch, _native
 from .gemm import layout_code
 
-KERNELS = {"auto": _native.KERNEL_AUTO, "tcgen05": _native.KERNEL_TCGEN05, "simt": _native.KERNEL_SIMT}
+KERNELS = {"auto": _native.KERNEL_AUTO, "tcgen05": _native.KERNEL_TCGEN05, "simt": _native.KERNEL_SIMT,
+           "pair": _native.KERNEL_GROUPED_PAIR, "split": _native.KERNEL_GROUPED_SPLIT}
+_GRADIENT_KERNELS = {name: KERNELS[name] for name in ("auto", "tcgen05", "simt")}
 
 _BF16 = (torch.bfloat16,)
 
@@ -47,7 +49,10 @@ def grouped_gemm(
 ) -> torch.Tensor:
     """Each row of ``x`` ``[rows, K]`` times its group's weight: ``[rows, N]``.
 
-    Rows may be strided; FP32 sums, one rounding.  Asynchronous on ``stream``
+    Rows may be strided; FP32 sums, one rounding.  ``kernel`` is ``"auto"``,
+    ``"tcgen05"`` (``"pair"`` or ``"split"`` by size: CTA pairs, or clusters that
+    split K for few rows; 16-byte aligned rows) or ``"simt"`` (any operands).
+    Asynchronous on ``stream``
     (the current one by default).  ``status`` is as for
     :func:`kernel_mcts_b200.gemm.bf16_gemm`.
     """
@@ -119,7 +124,7 @@ def grouped_gemm_wgrad(
     if accumulate and (out is None or dtype != torch.float32):
         raise ValueError("accumulate needs a float32 out")
     status_ptr = _launch.status_pointer(status, device)
-    kernel_id = kernel_code(kernel)
+    kernel_id = kernel_code(kernel, _GRADIENT_KERNELS)
     caller = _launch.caller_stream(device, stream)
     with _launch.on_device(device, stream):
         if out is None:

@@ -36,8 +36,12 @@ extern "C" {
 
 #define KMCTS_GROUPED_ZERO_REST 1 /* flags: zero the rows behind the last group */
 
-/* kernel: KMCTS_KERNEL_AUTO picks by size and alignment; KMCTS_KERNEL_SIMT is
- * the CUDA-core kernel, which takes any stride and alignment. */
+/* kernel: KMCTS_KERNEL_AUTO picks by size and alignment, KMCTS_KERNEL_TCGEN05
+ * by size among the tensor-core kernels, KMCTS_KERNEL_SIMT is the CUDA-core
+ * kernel, which takes any stride and alignment.  The forward products have two
+ * tensor-core kernels: CTA pairs, and clusters that split K for few rows. */
+#define KMCTS_KERNEL_GROUPED_PAIR 3
+#define KMCTS_KERNEL_GROUPED_SPLIT 4
 
 /* Element types of quantiser inputs, restored values and gradients. */
 #define KMCTS_TYPE_BF16 0

@@ -18,7 +18,8 @@ from kernel_mcts_b200 import _native, grouped
 
 pytestmark = pytest.mark.gpu
 
-KERNELS = ["auto", "simt"]
+KERNELS = ["auto", "pair", "split", "simt"]
+GRADIENT_KERNELS = ["auto", "simt"]
 
 # Row counts by group: empty groups at both ends and between, single rows,
 # lengths around the tiles' edges.
@@ -90,6 +91,10 @@ def test_forward_integers_bit_exact(cuda_device, kernel, layout, counts, n, k):
     rows = sum(counts) + 5  # five rows behind the last group
     x = integers(rows, k, seed=1)
     w = integers(len(counts), *((n, k) if layout == "col" else (k, n)), seed=2)
+    if kernel in ("pair", "split") and (k % 8 or (layout == "row" and n % 8)):
+        with pytest.raises(_native.KmctsError, match="not_supported"):  # rows that TMA cannot address
+            grouped.grouped_gemm(x, w, ends_of(counts), w_layout=layout, kernel=kernel)
+        return
     y = checked(grouped.grouped_gemm, x, w, ends_of(counts), w_layout=layout, kernel=kernel)
     ref, _ = forward64(x, w, counts, layout)
     assert torch.equal(y, ref.to(torch.bfloat16))
@@ -124,6 +129,7 @@ def test_rows_of_other_groups_and_behind_the_last_do_not_enter(cuda_device, kern
     dy = integers(len(x), n, seed=7)
     x[20:57] = integers(37, k, seed=8)
     dy[-9:] = float("nan")
+    kernel = kernel if kernel in GRADIENT_KERNELS else "auto"
     dw = checked(grouped.grouped_gemm_wgrad, dy, x, ends_of(counts), kernel=kernel)
     assert torch.equal(dw, wgrad64(dy, x, counts)[0].to(torch.bfloat16))
     # One group's NaN stays in its own gradient, whichever side of a boundary it is.
@@ -169,7 +175,7 @@ def test_ends_out_of_order_or_range_are_clamped(cuda_device, kernel):
     y = checked(grouped.grouped_gemm, x, w, ends, kernel=kernel)
     counts = [50, 0, 150, 0, 0]
     assert torch.equal(y, forward64(x, w, counts, "col")[0].to(torch.bfloat16))
-    dw = checked(grouped.grouped_gemm_wgrad, x, x, ends, kernel=kernel)
+    dw = checked(grouped.grouped_gemm_wgrad, x, x, ends, kernel=kernel if kernel in GRADIENT_KERNELS else "auto")
     assert torch.equal(dw, wgrad64(x, x, counts)[0].to(torch.bfloat16))
 
 
@@ -183,7 +189,7 @@ def test_many_groups(cuda_device):
     assert within(dw, ref, mag, 5, 2.0 ** -24)
 
 
-@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kernel", GRADIENT_KERNELS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("counts", COUNTS.values(), ids=COUNTS)
 @pytest.mark.parametrize("n,k", SIZES)
@@ -194,7 +200,7 @@ def test_wgrad_integers_bit_exact(cuda_device, kernel, dtype, counts, n, k):
     assert torch.equal(dw, wgrad64(dy, x, counts)[0].to(dtype))
 
 
-@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kernel", GRADIENT_KERNELS)
 def test_wgrad_normals_within_bound(cuda_device, kernel):
     counts, n, k = [70, 0, 2000, 1], 136, 264
     dy, x = normals(sum(counts), n, seed=3), normals(sum(counts), k, seed=4)
@@ -203,7 +209,7 @@ def test_wgrad_normals_within_bound(cuda_device, kernel):
         assert within(dw, *wgrad64(dy, x, counts), max(counts), half)
 
 
-@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kernel", GRADIENT_KERNELS)
 def test_wgrad_accumulates_into_fp32(cuda_device, kernel):
     counts, n, k = [70, 0, 130, 1], 136, 200
     dy, x = integers(sum(counts), n, seed=3), integers(sum(counts), k, seed=4)
@@ -316,6 +322,8 @@ def test_refusals(cuda_device):
         grouped.grouped_gemm(x[:1].expand(6, 16), w, ends)
     with pytest.raises(ValueError, match="kernel"):
         grouped.grouped_gemm(x, w, ends, kernel="fast")
+    with pytest.raises(ValueError, match="kernel"):
+        grouped.grouped_gemm_wgrad(x, x, ends, kernel="split")
     with pytest.raises(ValueError, match="status"):
         grouped.grouped_gemm(x, w, ends, status=torch.zeros(1, device="cuda"))
     with pytest.raises(ValueError, match="rows"):

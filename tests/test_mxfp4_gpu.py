@@ -18,7 +18,7 @@ from kernel_mcts_b200.mxfp4 import MXFP4Tensor
 
 pytestmark = pytest.mark.gpu
 
-KERNELS = ["auto", "simt"]
+KERNELS = ["auto", "pair", "split", "simt"]
 LEVELS = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
 
 
