@@ -7,7 +7,7 @@
 // contiguous part of K, so that few tiles still keep every SM busy and no
 // workspace is needed.  The CTAs' FP32 parts meet in shared memory: quarter q
 // of the tile's rows belongs to CTA q % S, every CTA stores its part of the
-// quarter there (plain stores to cluster shared memory), and the owner adds
+// quarter there (asynchronous stores, counted in bytes), and the owner adds
 // the S parts in K order, rounds once and writes 64-byte pieces of token rows.
 // The order of the sum is fixed, so repeated calls give the same bits.
 //
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
         }
         ptx::mbar_init(drain, 1);
         ptx::mbar_init(copies_done, 1);
-        ptx::mbar_init(arrived, 4);
+        ptx::mbar_init(arrived, 1);
         for (int q = 0; q < 4; ++q) ptx::mbar_init(&freed[q], 4);
         *abort = 0;
         *no_abort = 0;
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
                 ok = ptx::mbar_wait(&tmem_full[acc], (local >> 1) & 1, p.limit_ns, abort);
                 ++local;
             }
-            if (ok && seen > 0) ok = ptx::mbar_wait_cluster(&freed[quarter], (seen - 1) & 1, p.limit_ns, abort);
+            if (ok && seen > 0) ok = ptx::mbar_wait(&freed[quarter], (seen - 1) & 1, p.limit_ns, abort);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) record_failure(p.status, abort, kRoleEpilogue);
                 break;
@@ -291,19 +291,18 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
 #pragma unroll
                 for (int g = 0; g < 8; ++g)
                     if (c + 4 * g < w.width)
-                        ptx::st_cluster_v4(mine + (c / 4 + g) * 512, __uint_as_float(r[4 * g]),
-                                           __uint_as_float(r[4 * g + 1]), __uint_as_float(r[4 * g + 2]),
-                                           __uint_as_float(r[4 * g + 3]));
+                        ptx::st_async_v4(mine + (c / 4 + g) * 512, r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3],
+                                         mine_arrived);
             }
             if (computed) {
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&tmem_empty[acc]);
             }
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_release_cluster(mine_arrived);
+            // Four parts of width x 32 values come here, whatever S is.
+            if (threadIdx.x == 64) ptx::mbar_arrive_expect_tx(arrived, static_cast<uint32_t>(w.width * 512));
             // The parts of this CTA's quarters: the four warps share the tokens.
-            ok = __all_sync(0xffffffffu, ptx::mbar_wait_cluster(arrived, seen & 1, p.limit_ns, abort));
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(arrived, seen & 1, p.limit_ns, abort));
             if (!ok) {
                 if (lane == 0) record_failure(p.status, abort, kRoleEpilogue);
                 break;
@@ -323,9 +322,11 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
                     for (int j = 0; j < 4; ++j)
                         if (col < p.n && 4 * g + j < w.valid) dst[j * p.ldy] = __float2bfloat16_rn(values[j]);
                 }
+                // The parts have been read (their sums are stored), which is
+                // all that the next ones wait for: no release of the stores
+                // to Y, which would wait for memory.
                 __syncwarp();
-                if (lane < splits)
-                    ptx::mbar_arrive_release_cluster(ptx::mapa_shared(ptx::smem_addr(&freed[q]), lane));
+                if (lane < splits) ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_addr(&freed[q]), lane));
             }
         }
         __syncwarp();

@@ -48,6 +48,16 @@ __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, const void* s
         : "memory");
 }
 
+// Asynchronous 16-byte store into the shared memory of any CTA of the cluster;
+// its bytes are counted on an mbarrier of that CTA (both from mapa_shared).
+__device__ __forceinline__ void st_async_v4(uint32_t cluster_addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d,
+                                            uint32_t bar_cluster_addr) {
+    asm volatile(
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(cluster_addr),
+        "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar_cluster_addr)
+        : "memory");
+}
+
 // Each of the 32 rows of 16 bytes at `desc` goes to one TMEM lane of four
 // consecutive columns at `taddr`, repeated in all four lane quarters.
 template <int CTAS>
