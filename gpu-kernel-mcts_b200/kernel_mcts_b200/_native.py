@@ -182,6 +182,8 @@ def library_path() -> Path:
 def load() -> ctypes.CDLL:
     """Loads (once) and returns the native library."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

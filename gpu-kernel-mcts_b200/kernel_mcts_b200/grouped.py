@@ -27,6 +27,7 @@ KERNELS = {"auto": _native.KERNEL_AUTO, "tcgen05": _native.KERNEL_TCGEN05, "simt
 _GRADIENT_KERNELS = {name: KERNELS[name] for name in ("auto", "tcgen05", "simt")}
 
 _BF16 = (torch.bfloat16,)
+_GRADIENT_TYPES = {torch.bfloat16: _native.TYPE_BF16, torch.float32: _native.TYPE_FP32}
 
 
 def kernel_code(kernel: str, kernels: dict[str, int] = KERNELS) -> int:
@@ -57,35 +58,32 @@ def grouped_gemm(
     :func:`kernel_mcts_b200.gemm.bf16_gemm`.
     """
     code = layout_code(w_layout)
-    device = x.device
-    _launch.check_tensor("x", x, 2, _BF16)
-    _launch.check_tensor("w", w, 3, _BF16, device)
+    device = x.get_device()
+    (rows, k), _, ldx = _launch.rows_of("x", x, 2, _BF16, device, 8)
+    w_shape, w_strides, ldw = _launch.rows_of("w", w, 3, _BF16, device, 8)
     groups = _launch.check_groups(ends, device)
-    rows, k = x.shape
-    n, kw = (w.shape[1], w.shape[2]) if code == _native.B_COL else (w.shape[2], w.shape[1])
+    n, kw = (w_shape[1], w_shape[2]) if code == _native.B_COL else (w_shape[2], w_shape[1])
     if kw != k:
         raise ValueError(f"inner dimensions differ: x has K={k}, w has K={kw}")
-    if w.shape[0] != groups:
-        raise ValueError(f"w holds {w.shape[0]} groups, ends {groups}")
-    ldx, ldw = _launch.row_stride("x", x, 0, 8), _launch.row_stride("w", w, 1, 8)
+    if w_shape[0] != groups:
+        raise ValueError(f"w holds {w_shape[0]} groups, ends {groups}")
     status_ptr = _launch.status_pointer(status, device)
     kernel_id = kernel_code(kernel)
     caller = _launch.caller_stream(device, stream)
     with _launch.on_device(device, stream):
-        flags = 0
         if out is None:
-            out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
-            _launch.share_result(out, caller)
-            flags = _native.GROUPED_ZERO_REST
+            out = _launch.share_result(x.new_empty((rows, n)), caller)
+            ldy, flags = n, _native.GROUPED_ZERO_REST
         else:
-            _launch.check_tensor("out", out, 2, _BF16, device)
-            if out.shape[0] != rows or out.shape[1] != n:
-                raise ValueError(f"out must have shape {(rows, n)}, got {tuple(out.shape)}")
+            shape, _, ldy = _launch.rows_of("out", out, 2, _BF16, device, 8)
+            if shape != (rows, n):
+                raise ValueError(f"out must have shape {(rows, n)}, got {tuple(shape)}")
+            flags = 0
         rc = _native.load().kmcts_bf16_grouped_gemm(
-            x.data_ptr(), ldx, w.data_ptr(), w.stride(0) if groups > 1 else 0, ldw, code, out.data_ptr(),
-            _launch.row_stride("out", out, 0, 8), ends.data_ptr(), groups, rows, n, k, flags, kernel_id,
-            _launch.stream_handle(device, stream), status_ptr)
-    _native.check(rc, "kmcts_bf16_grouped_gemm")
+            x.data_ptr(), ldx, w.data_ptr(), w_strides[0] if groups > 1 else 0, ldw, code, out.data_ptr(), ldy,
+            ends.data_ptr(), groups, rows, n, k, flags, kernel_id, _launch.stream_handle(device), status_ptr)
+    if rc:
+        _native.check(rc, "kmcts_bf16_grouped_gemm")
     return out
 
 
@@ -108,18 +106,15 @@ def grouped_gemm_wgrad(
     several micro-batches; an empty group then leaves its part as it was, and
     is zeros otherwise.
     """
-    device = dy.device
-    _launch.check_tensor("dy", dy, 2, _BF16)
-    _launch.check_tensor("x", x, 2, _BF16, device)
+    device = dy.get_device()
+    (rows, n), _, lddy = _launch.rows_of("dy", dy, 2, _BF16, device, 8)
+    (x_rows, k), _, ldx = _launch.rows_of("x", x, 2, _BF16, device, 8)
     groups = _launch.check_groups(ends, device)
-    rows, n = dy.shape
-    k = x.shape[1]
-    if x.shape[0] != rows:
-        raise ValueError(f"dy has {rows} rows, x {x.shape[0]}")
-    lddy, ldx = _launch.row_stride("dy", dy, 0, 8), _launch.row_stride("x", x, 0, 8)
+    if x_rows != rows:
+        raise ValueError(f"dy has {rows} rows, x {x_rows}")
     if dtype is None:
         dtype = out.dtype if out is not None else torch.bfloat16
-    if dtype not in (torch.bfloat16, torch.float32):
+    if dtype not in _GRADIENT_TYPES:
         raise TypeError(f"the gradient must be bfloat16 or float32, got {dtype}")
     if accumulate and (out is None or dtype != torch.float32):
         raise ValueError("accumulate needs a float32 out")
@@ -128,21 +123,20 @@ def grouped_gemm_wgrad(
     caller = _launch.caller_stream(device, stream)
     with _launch.on_device(device, stream):
         if out is None:
-            out = torch.empty((groups, n, k), dtype=dtype, device=device)
-            _launch.share_result(out, caller)
+            out = _launch.share_result(x.new_empty((groups, n, k), dtype=dtype), caller)
+            ldo, group_stride = k, n * k
         else:
-            _launch.check_tensor("out", out, 3, (dtype,), device)
-            if tuple(out.shape) != (groups, n, k):
-                raise ValueError(f"out must have shape {(groups, n, k)}, got {tuple(out.shape)}")
-        ldo = _launch.row_stride("out", out, 1, 8)
-        group_stride = out.stride(0) if groups > 1 else n * ldo
-        if groups > 1 and n > 0 and group_stride < (n - 1) * ldo + k:
-            raise ValueError("out has overlapping groups")
+            shape, strides, ldo = _launch.rows_of("out", out, 3, (dtype,), device, 8)
+            if shape != (groups, n, k):
+                raise ValueError(f"out must have shape {(groups, n, k)}, got {tuple(shape)}")
+            group_stride = strides[0] if groups > 1 else n * ldo
+            if groups > 1 and n > 0 and group_stride < (n - 1) * ldo + k:
+                raise ValueError("out has overlapping groups")
         rc = _native.load().kmcts_bf16_grouped_wgrad(
-            dy.data_ptr(), lddy, x.data_ptr(), ldx, out.data_ptr(), group_stride, ldo,
-            _native.TYPE_FP32 if dtype == torch.float32 else _native.TYPE_BF16, int(accumulate), ends.data_ptr(), groups,
-            rows, n, k, kernel_id, _launch.stream_handle(device, stream), status_ptr)
-    _native.check(rc, "kmcts_bf16_grouped_wgrad")
+            dy.data_ptr(), lddy, x.data_ptr(), ldx, out.data_ptr(), group_stride, ldo, _GRADIENT_TYPES[dtype],
+            int(accumulate), ends.data_ptr(), groups, rows, n, k, kernel_id, _launch.stream_handle(device), status_ptr)
+    if rc:
+        _native.check(rc, "kmcts_bf16_grouped_wgrad")
     return out
 
 

@@ -23,6 +23,8 @@ _TYPES = {
     torch.float16: _native.TYPE_FP16,
     torch.float32: _native.TYPE_FP32,
 }
+_TYPE_TUPLE = tuple(_TYPES)
+_BF16 = (torch.bfloat16,)
 _CODES = (torch.uint8, torch.float4_e2m1fn_x2)
 _SCALES = (torch.uint8, torch.float8_e8m0fnu)
 
@@ -38,15 +40,17 @@ class MXFP4Tensor(NamedTuple):
         return (*self.codes.shape[:-1], 2 * self.codes.shape[-1])
 
 
-def _check_pair(name: str, q: MXFP4Tensor, dims: int, device: torch.device | None = None) -> None:
-    _launch.check_tensor(f"{name} codes", q.codes, dims, _CODES, device)
-    _launch.check_tensor(f"{name} scales", q.scales, dims, _SCALES, q.codes.device)
-    k = 2 * q.codes.shape[-1]
-    if k % BLOCK != 0:
-        raise ValueError(f"{name} has K={k}, not a multiple of {BLOCK}")
-    want = (*q.codes.shape[:-1], k // BLOCK)
-    if tuple(q.scales.shape) != want:
-        raise ValueError(f"{name} scales must have shape {want}, got {tuple(q.scales.shape)}")
+def _pair_rows(name: str, q: MXFP4Tensor, dims: int, index: int):
+    """(code shape, code strides, code row stride, scale strides, scale row
+    stride) of a checked pair."""
+    shape, strides, ldc = _launch.rows_of(f"{name} codes", q[0], dims, _CODES, index, 16)
+    scale_shape, scale_strides, lds = _launch.rows_of(f"{name} scales", q[1], dims, _SCALES, index, 1)
+    if shape[-1] % (BLOCK // 2) != 0:
+        raise ValueError(f"{name} has K={2 * shape[-1]}, not a multiple of {BLOCK}")
+    if scale_shape[-1] != shape[-1] // (BLOCK // 2) or scale_shape[:-1] != shape[:-1]:
+        want = (*shape[:-1], shape[-1] // (BLOCK // 2))
+        raise ValueError(f"{name} scales must have shape {want}, got {tuple(scale_shape)}")
+    return shape, strides, ldc, scale_strides, lds
 
 
 def _rows(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -72,31 +76,29 @@ def mxfp4_quantize(
     even, and saturate at 6 scales.  A block that holds an infinity or a NaN
     gets the NaN scale; its codes mean nothing.
     """
-    if x.dim() < 1 or x.shape[-1] % BLOCK != 0:
-        raise ValueError(f"x must have a last dimension that is a multiple of {BLOCK}, got shape {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] % BLOCK != 0:
+        raise ValueError(f"x must have a last dimension that is a multiple of {BLOCK}, got shape {tuple(shape)}")
     flat = _rows("x", x)
-    _launch.check_tensor("x", flat, 2, tuple(_TYPES))
-    device = x.device
-    rows, k = flat.shape
-    ldx = _launch.row_stride("x", flat, 0, BLOCK)
+    device = x.get_device()
+    (rows, k), _, ldx = _launch.rows_of("x", flat, 2, _TYPE_TUPLE, device, BLOCK)
     caller = _launch.caller_stream(device, stream)
     with _launch.on_device(device, stream):
         if out is None:
-            lead = x.shape[:-1]
-            out = MXFP4Tensor(torch.empty((*lead, k // 2), dtype=torch.uint8, device=device),
-                              torch.empty((*lead, k // BLOCK), dtype=torch.uint8, device=device))
-            for t in out:
-                _launch.share_result(t, caller)
+            lead = shape[:-1]
+            codes = _launch.share_result(x.new_empty((*lead, k // 2), dtype=torch.uint8), caller)
+            scales = _launch.share_result(x.new_empty((*lead, k // BLOCK), dtype=torch.uint8), caller)
+            out, ldc, lds = MXFP4Tensor(codes, scales), k // 2, k // BLOCK
         else:
-            _check_pair("out", out, x.dim(), device)
-            if out.shape != tuple(x.shape):
-                raise ValueError(f"out must have shape {tuple(x.shape)}, got {out.shape}")
-        codes, scales = _rows("out codes", out.codes), _rows("out scales", out.scales)
+            codes, scales = _rows("out codes", out.codes), _rows("out scales", out.scales)
+            _, _, ldc, _, lds = _pair_rows("out", MXFP4Tensor(codes, scales), 2, device)
+            if out.shape != tuple(shape):
+                raise ValueError(f"out must have shape {tuple(shape)}, got {out.shape}")
         rc = _native.load().kmcts_mxfp4_quantize(
-            flat.data_ptr(), _TYPES[x.dtype], ldx, codes.data_ptr(), _launch.row_stride("out codes", codes, 0, 16),
-            scales.data_ptr(), _launch.row_stride("out scales", scales, 0, 1), rows, k,
-            _launch.stream_handle(device, stream))
-    _native.check(rc, "kmcts_mxfp4_quantize")
+            flat.data_ptr(), _TYPES[x.dtype], ldx, codes.data_ptr(), ldc, scales.data_ptr(), lds, rows, k,
+            _launch.stream_handle(device))
+    if rc:
+        _native.check(rc, "kmcts_mxfp4_quantize")
     return out
 
 
@@ -109,29 +111,31 @@ def mxfp4_dequantize(
 ) -> torch.Tensor:
     """The values of ``q`` in ``dtype`` (``out``'s type, or bfloat16), rounded
     once; exact in float32, and in bfloat16 from ``2^-133`` up."""
-    _check_pair("q", q, q.codes.dim())
-    device = q.codes.device
+    codes, scales = _rows("q codes", q[0]), _rows("q scales", q[1])
+    device = codes.get_device()
+    (rows, half), _, ldc, _, lds = _pair_rows("q", MXFP4Tensor(codes, scales), 2, device)
+    if q.scales.shape[:-1] != q.codes.shape[:-1]:
+        raise ValueError(f"q scales must go with codes of shape {tuple(q.codes.shape)}, got {tuple(q.scales.shape)}")
+    k = 2 * half
     if dtype is None:
         dtype = out.dtype if out is not None else torch.bfloat16
     if dtype not in _TYPES:
         raise TypeError(f"values must be bfloat16, float16 or float32, got {dtype}")
-    codes, scales = _rows("codes", q.codes), _rows("scales", q.scales)
-    rows, k = codes.shape[0], 2 * codes.shape[1]
-    ldc, lds = _launch.row_stride("codes", codes, 0, 16), _launch.row_stride("scales", scales, 0, 1)
     caller = _launch.caller_stream(device, stream)
     with _launch.on_device(device, stream):
         if out is None:
-            out = torch.empty(q.shape, dtype=dtype, device=device)
-            _launch.share_result(out, caller)
+            flat = out = _launch.share_result(codes.new_empty(q.shape, dtype=dtype), caller)
+            ldo = k
         else:
-            _launch.check_tensor("out", out, q.codes.dim(), (dtype,), device)
             if tuple(out.shape) != q.shape:
                 raise ValueError(f"out must have shape {q.shape}, got {tuple(out.shape)}")
-        flat = _rows("out", out)
+            flat = _rows("out", out)
+            _, _, ldo = _launch.rows_of("out", flat, 2, (dtype,), device, BLOCK)
         rc = _native.load().kmcts_mxfp4_dequantize(
-            codes.data_ptr(), ldc, scales.data_ptr(), lds, flat.data_ptr(), _TYPES[dtype],
-            _launch.row_stride("out", flat, 0, BLOCK), rows, k, _launch.stream_handle(device, stream))
-    _native.check(rc, "kmcts_mxfp4_dequantize")
+            codes.data_ptr(), ldc, scales.data_ptr(), lds, flat.data_ptr(), _TYPES[dtype], ldo, rows, k,
+            _launch.stream_handle(device))
+    if rc:
+        _native.check(rc, "kmcts_mxfp4_dequantize")
     return out
 
 
@@ -151,39 +155,36 @@ def mxfp4_gemm(
     ``ends``, ``b`` is ``[groups, N, K]`` and each row of ``a`` meets its own
     group's weight, as in :func:`kernel_mcts_b200.grouped.grouped_gemm`.
     """
-    device = a.codes.device
-    _check_pair("a", a, 2)
-    _check_pair("b", b, 2 if ends is None else 3, device)
-    rows, k = a.codes.shape[0], 2 * a.codes.shape[1]
-    if 2 * b.codes.shape[-1] != k:
-        raise ValueError(f"inner dimensions differ: a has K={k}, b has K={2 * b.codes.shape[-1]}")
-    n = b.codes.shape[-2]
-    groups, ends_ptr = 1, None
+    device = a[0].get_device()
+    (rows, half), _, lda, _, ldas = _pair_rows("a", a, 2, device)
+    b_shape, b_strides, ldb, bs_strides, ldbs = _pair_rows("b", b, 2 if ends is None else 3, device)
+    if b_shape[-1] != half:
+        raise ValueError(f"inner dimensions differ: a has K={2 * half}, b has K={2 * b_shape[-1]}")
+    k, n = 2 * half, b_shape[-2]
+    groups, ends_ptr, b_stride, bs_stride = 1, None, 0, 0
     if ends is not None:
         groups, ends_ptr = _launch.check_groups(ends, device), ends.data_ptr()
-        if b.codes.shape[0] != groups:
-            raise ValueError(f"b holds {b.codes.shape[0]} groups, ends {groups}")
-    lda, ldas = _launch.row_stride("a codes", a.codes, 0, 16), _launch.row_stride("a scales", a.scales, 0, 1)
-    ldb, ldbs = _launch.row_stride("b codes", b.codes, -2, 16), _launch.row_stride("b scales", b.scales, -2, 1)
-    strides = (b.codes.stride(0), b.scales.stride(0)) if groups > 1 else (0, 0)
+        if b_shape[0] != groups:
+            raise ValueError(f"b holds {b_shape[0]} groups, ends {groups}")
+        if groups > 1:
+            b_stride, bs_stride = b_strides[0], bs_strides[0]
     status_ptr = _launch.status_pointer(status, device)
     kernel_id = kernel_code(kernel)
     caller = _launch.caller_stream(device, stream)
     with _launch.on_device(device, stream):
-        flags = 0
         if out is None:
-            out = torch.empty((rows, n), dtype=torch.bfloat16, device=device)
-            _launch.share_result(out, caller)
-            flags = _native.GROUPED_ZERO_REST
+            out = _launch.share_result(a[1].new_empty((rows, n), dtype=torch.bfloat16), caller)
+            ldy, flags = n, _native.GROUPED_ZERO_REST
         else:
-            _launch.check_tensor("out", out, 2, (torch.bfloat16,), device)
-            if out.shape[0] != rows or out.shape[1] != n:
-                raise ValueError(f"out must have shape {(rows, n)}, got {tuple(out.shape)}")
+            shape, _, ldy = _launch.rows_of("out", out, 2, _BF16, device, 8)
+            if shape != (rows, n):
+                raise ValueError(f"out must have shape {(rows, n)}, got {tuple(shape)}")
+            flags = 0
         rc = _native.load().kmcts_mxfp4_gemm(
-            a.codes.data_ptr(), lda, a.scales.data_ptr(), ldas, b.codes.data_ptr(), strides[0], ldb,
-            b.scales.data_ptr(), strides[1], ldbs, out.data_ptr(), _launch.row_stride("out", out, 0, 8), ends_ptr, groups,
-            rows, n, k, flags, kernel_id, _launch.stream_handle(device, stream), status_ptr)
-    _native.check(rc, "kmcts_mxfp4_gemm")
+            a[0].data_ptr(), lda, a[1].data_ptr(), ldas, b[0].data_ptr(), b_stride, ldb, b[1].data_ptr(), bs_stride, ldbs,
+            out.data_ptr(), ldy, ends_ptr, groups, rows, n, k, flags, kernel_id, _launch.stream_handle(device), status_ptr)
+    if rc:
+        _native.check(rc, "kmcts_mxfp4_gemm")
     return out
 
 
