@@ -1,8 +1,6 @@
 // C entry points of the grouped products (declared in include/kmcts_grouped.h).
 #include <cudaTypedefs.h>
 
-#include <cstdlib>
-
 #include <mutex>
 
 #include "grouped_tiles.cuh"
@@ -72,11 +70,31 @@ bool bad_groups(const int32_t* ends, int groups, int rows, int n, int k) {
     return rows < 0 || n < 0 || k < 0 || groups < 1 || groups > KMCTS_MAX_GROUPS || !ends;
 }
 
-// CTAs that share a tile of the few-rows kernel, or 0 for the pair kernel.
-int few_row_splits(const ForwardArgs& a) {
-    static const char* env = getenv("KSPLIT");
-    if (env) return atoi(env);
-    return a.rows <= 32LL * a.groups ? 4 : 0;
+// Whether the few-rows kernel should take a product, and how many CTAs share
+// one of its tiles (128 weight rows x 64 tokens; how many there are is known
+// up to where the groups end).  GPU time on B200 with operands read from HBM,
+// pair / split in two / split in four:
+// * as many tiles as a quarter of the SMs or fewer: four (64 x 4096 x 4096 BF16
+//   25.6 / 18.1 / 13.7 us, MXFP4 12.7 / 11.7 / 10.2);
+// * up to half the SMs: two, one round of tiles (128 x 4096 x 4096 BF16 26.9 /
+//   18.5 / 18.2, MXFP4 13.9 / 12.1 / 13.2; past it pairs win: 512 x 4096 x 4096
+//   29.5 / 48.9 / 49.7);
+// * more tiles, few rows a group on average: two, whose finer tiles share the
+//   SMs evenly while the weights stream in (64 experts of 2048 x 4096, 256 rows
+//   180 / 166 / 185; 16 of 4096 x 4096, 512 rows 110 / 91 / -, 768 rows 111 /
+//   110, 1024 rows 111 / 117; MXFP4 32 of 2048 x 4096, 1024 rows 37.7 / 35.4,
+//   1500 rows 39.0 / 42.5).
+struct FewRows {
+    bool better;
+    int splits;
+};
+
+FewRows few_rows(const ForwardArgs& a) {
+    const int64_t used = a.groups < a.rows ? a.groups : a.rows;
+    const int64_t tiles = ((a.rows + 63) / 64 + used - 1) * ((a.n + 127) / 128);
+    const int sms = multiprocessor_count();
+    if (4 * tiles <= sms) return {true, 4};
+    return {2 * tiles <= sms || a.rows <= 40LL * a.groups, 2};
 }
 
 int forward(const ForwardArgs& a, Operand kind, int kernel, cudaStream_t stream, int* status) {
@@ -86,11 +104,10 @@ int forward(const ForwardArgs& a, Operand kind, int kernel, cudaStream_t stream,
     if (kernel != KMCTS_KERNEL_SIMT && a.k > 0) {
         if (!status) status = default_status_ptr();
         if (!status) return KMCTS_EHANDLE;
-        const int splits = kernel == KMCTS_KERNEL_GROUPED_PAIR   ? 0
-                           : kernel == KMCTS_KERNEL_GROUPED_SPLIT ? (few_row_splits(a) > 0 ? few_row_splits(a) : 2)
-                                                                  : few_row_splits(a);
-        const int rc = splits > 0 ? launch_forward_split(a, kind, splits, gemm::kDefaultWaitNs, stream, status)
-                                  : launch_forward_pair(a, kind, gemm::kDefaultWaitNs, stream, status);
+        const FewRows few = few_rows(a);
+        const bool split = kernel == KMCTS_KERNEL_GROUPED_SPLIT || (few.better && kernel != KMCTS_KERNEL_GROUPED_PAIR);
+        const int rc = split ? launch_forward_split(a, kind, few.splits, gemm::kDefaultWaitNs, stream, status)
+                             : launch_forward_pair(a, kind, gemm::kDefaultWaitNs, stream, status);
         if (rc != KMCTS_ENOTSUP || kernel != KMCTS_KERNEL_AUTO) return rc;
     }
     return launch_forward_simt(a, kind, stream);
