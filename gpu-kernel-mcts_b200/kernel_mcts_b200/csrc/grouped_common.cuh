@@ -62,19 +62,15 @@ __device__ __forceinline__ void build_group_table(const GroupTable& t, const int
     }
 }
 
-// The group that tile `t` belongs to: the last one whose first tile is <= t
-// and that is not empty.
-__device__ __forceinline__ int group_of_tile(const GroupTable& table, int t) {
-    int lo = 0, hi = table.groups;  // tile[lo] <= t < tile[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (table.tile[mid] <= t) {
-            lo = mid;
-        } else {
-            hi = mid;
-        }
-    }
-    return lo;
+// The group that tile `t` belongs to (the one group with tile[e] <= t <
+// tile[e + 1]).  A CTA's tiles come in increasing order, so the search goes on
+// from the last tile's group; a search from the start cost a tile more than
+// the steps that this takes over a whole launch.
+__device__ __forceinline__ int group_of_tile(const GroupTable& table, int t, int& last) {
+    int e = last;
+    while (table.tile[e + 1] <= t) ++e;
+    last = e;
+    return e;
 }
 
 // Zeroes the rows of Y behind the last group, spread over the whole grid.

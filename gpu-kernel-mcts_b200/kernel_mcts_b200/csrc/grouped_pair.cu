@@ -16,7 +16,7 @@
 // takes no further step.
 //
 // Roles per CTA: warp 0 TMA producer; warp 1 MMA (the pair's leader issues);
-// warps 2-5 epilogue; MXFP4 adds four warps that fetch scales and one that
+// warps 2-9 epilogue; MXFP4 adds four warps that fetch scales and one that
 // issues their copies into TMEM, the gradient one that zeroes tails.  Every CTA reads the groups' ends itself and walks
 // the tiles round-robin; nothing is decided on the host.  Every wait is
 // bounded.
@@ -29,7 +29,9 @@ namespace grouped {
 namespace {
 
 constexpr int kAccCols = 256;      // TMEM columns from one accumulator to the next (MXFP4: 192)
-constexpr int kBaseThreads = 192;  // producer, MMA, four epilogue warps
+constexpr int kEpilogueWarps = 8;  // two for each quarter of the TMEM lanes
+constexpr int kBaseThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kExtraWarp = kBaseThreads / 32;
 
 template <Kind KIND>
 struct Pair {
@@ -47,9 +49,9 @@ struct Pair {
     // MXFP4: each stage's scales have TMEM columns of their own, 8 + 16.
     static constexpr int kStages = kMx ? 5 : kGrad ? 5 : 6;
     static constexpr int kScaleCols = 24;
-    static constexpr int kStagingBytes = kGrad ? 8192 : 2048;  // an epilogue warp's
+    static constexpr int kStagingBytes = kGrad ? 4096 : 2048;  // an epilogue warp's
     static constexpr int kStagingOffset = kStages * kStageBytes;
-    static constexpr int kBarrierOffset = kStagingOffset + 4 * kStagingBytes;
+    static constexpr int kBarrierOffset = kStagingOffset + kEpilogueWarps * kStagingBytes;
     static constexpr int kTableOffset = kBarrierOffset + 512;
     static constexpr int smem_bytes(int groups) { return 1024 + kTableOffset + 8 * (groups + 1); }
     static_assert(2 * kMaxWidth + (kMx ? kStages * kScaleCols : 0) <= 512, "TMEM columns");
@@ -82,10 +84,10 @@ struct Tile {
 };
 
 template <Kind KIND>
-__device__ __forceinline__ Tile tile_at(const GroupTable& table, const PairParams& p, int t) {
+__device__ __forceinline__ Tile tile_at(const GroupTable& table, const PairParams& p, int t, int& group) {
     using L = Pair<KIND>;
     Tile out = {};
-    out.e = group_of_tile(table, t);
+    out.e = group_of_tile(table, t, group);
     const int in_group = t - table.tile[out.e];
     const int first = table.row[out.e], rows = table.row[out.e + 1] - first;
     if constexpr (L::kGrad) {
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
         }
         for (int a = 0; a < 2; ++a) {
             ptx::mbar_init(&bar.tmem_full[a], 1);
-            ptx::mbar_init(&bar.tmem_empty[a], 8);
+            ptx::mbar_init(&bar.tmem_empty[a], 2 * kEpilogueWarps);
         }
         ptx::mbar_init(bar.drain, 1);
         ptx::mbar_init(bar.copies_done, 1);
@@ -197,6 +199,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
     ptx::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int tiles = table.tiles();
+    int group = 0;  // the last tile's
     constexpr int kAccStep = L::kMx ? 192 : kAccCols;
 
     if (warp == 0) {
@@ -206,7 +209,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
             uint32_t issued = 0, issued_phase = 0;
             bool ok = true;
             for (int t = first_tile; t < tiles && ok; t += tile_step) {
-                const Tile w = tile_at<KIND>(table, p, t);
+                const Tile w = tile_at<KIND>(table, p, t, group);
                 const int half = w.width / 2;
                 const int a0 = w.n0 + rank * 128, b0 = w.b0 + rank * half;
                 // MN-major operands come in boxes of 64 columns, tokens in one
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
             int local = 0;
             bool ok = true;
             for (int t = first_tile; t < tiles && ok; t += tile_step) {
-                const Tile w = tile_at<KIND>(table, p, t);
+                const Tile w = tile_at<KIND>(table, p, t, group);
                 if (w.blocks == 0) continue;
                 const int acc = local & 1;
                 if (!ptx::mbar_wait(&bar.tmem_empty[acc], ((local >> 1) & 1) ^ 1u, p.limit_ns, abort)) {
@@ -332,13 +335,17 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
             ptx::umma_commit_pair(bar.drain, 3);
         }
         __syncwarp();
-    } else if (warp < 6) {
+    } else if (warp < kExtraWarp) {
         // ------------------------------------------------------------ epilogue
-        const int quarter = warp % 4;
+        // Two warps share a quarter's lanes and take its chunks of columns in
+        // turn.  (With one warp a quarter the epilogue was longer than the
+        // MMAs of a short contraction: 16 x 4096 x 4096 from 64 rows a group
+        // took 148 us, the weights' gradient of 512 rows a group 267.)
+        const int quarter = warp % 4, turn = (warp - 2) / 4;
         uint8_t* staging = smem + L::kStagingOffset + (warp - 2) * L::kStagingBytes;
-        int local = 0, stored = 0;
+        int local = 0;
         for (int t = first_tile; t < tiles; t += tile_step) {
-            const Tile w = tile_at<KIND>(table, p, t);
+            const Tile w = tile_at<KIND>(table, p, t, group);
             const bool computed = w.blocks != 0;
             if (!computed && p.accumulate) continue;  // adds nothing
             const int acc = local & 1;
@@ -354,71 +361,87 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
             const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
                                    static_cast<uint32_t>(acc * kAccStep);
             const int n0 = w.n0 + rank * 128 + quarter * 32;
+            if constexpr (!L::kGrad) {
 #pragma unroll 1
-            for (int c = 0; c < w.width; c += 32) {
-                uint32_t r[32];
-                if (computed) {
-                    ptx::tmem_ld_32x32b_x32(lanes + c, r);
-                    ptx::tmem_wait_ld();
-                    if (c + 32 >= w.width) {
-                        ptx::tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.tmem_empty[acc]), 0));
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) r[j] = 0;
-                }
-                if constexpr (!L::kGrad) {
+                for (int c = 32 * turn; c < w.width; c += 64) {
+                    uint32_t r[32];
+                    load_rows_of_8(lanes + c, r);
                     store_transposed(r, staging, p.y + static_cast<int64_t>(w.b0 + c) * p.ldy, p.ldy, w.valid - c, n0, p.n,
                                      p.vec, lane);
-                } else {
-                    // Lanes are rows of the gradient: 32 rows of 128 bytes (64
-                    // columns, 32 in FP32) go through a swizzled buffer and
-                    // out by TMA, which clips them at the group's own edges.
-                    // (64-byte rows of BF16 took twice as long as the MMAs at
-                    // 512 rows a group: 311 us for 16 x 4096 x 4096.)
-                    const bool second = !p.fp32 && (c & 32);
-                    uint8_t* buf = staging + (stored & 1) * 4096;
-                    if (!second) {
-                        if (lane == 0) ptx::bulk_wait_group_read<1>();
-                        __syncwarp();
+                }
+            } else {
+                // Lanes are rows of the gradient: 32 rows of 128 bytes (64
+                // columns, 32 in FP32) go through a swizzled buffer and out by
+                // TMA, which clips them at the group's own edges: columns of a
+                // last chunk past the width are past the row's end too.
+                // (64-byte rows of BF16 took 311 us for 16 groups of 512 rows,
+                // 4096 x 4096.)
+                auto send = [&](int col) {
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && n0 < p.n && col < p.k) {
+                        if (p.accumulate)
+                            ptx::tma_add_3d(&map_c, staging, col, n0, w.e);
+                        else
+                            ptx::tma_store_3d(&map_c, staging, col, n0, w.e);
+                        ptx::bulk_commit_group();
                     }
+                };
+                auto reusable = [&] {
+                    if (lane == 0) ptx::bulk_wait_group_read<0>();
+                    __syncwarp();
+                };
+#pragma unroll 1
+                for (int c = 64 * turn; c < w.width; c += 128) {
+                    uint32_t lo[32], hi[32];
+                    if (computed) {
+                        ptx::tmem_ld_32x32b_x32(lanes + c, lo);
+                        ptx::tmem_ld_32x32b_x32(lanes + c + 32, hi);
+                        ptx::tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) lo[j] = hi[j] = 0;
+                    }
+                    uint8_t* row = staging + lane * 128;
+                    reusable();
                     if (p.fp32) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<uint4*>(buf + lane * 128 + (j ^ (lane & 7)) * 16) =
-                                make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                            *reinterpret_cast<uint4*>(row + (j ^ (lane & 7)) * 16) =
+                                make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
+                        send(w.b0 + c);
+                        reusable();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<uint4*>(row + (j ^ (lane & 7)) * 16) =
+                                make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
+                        send(w.b0 + c + 32);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            *reinterpret_cast<uint4*>(buf + lane * 128 + ((j + (second ? 4 : 0)) ^ (lane & 7)) * 16) =
-                                make_uint4(gemm::pack_bf16x2(r[8 * j], r[8 * j + 1]),
-                                           gemm::pack_bf16x2(r[8 * j + 2], r[8 * j + 3]),
-                                           gemm::pack_bf16x2(r[8 * j + 4], r[8 * j + 5]),
-                                           gemm::pack_bf16x2(r[8 * j + 6], r[8 * j + 7]));
-                        // A last half chunk's other half lies past the row's end.
-                        if (!second && c + 32 < w.width) continue;
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t(&half)[32] = j < 4 ? lo : hi;
+                            const int at = j % 4 * 8;
+                            *reinterpret_cast<uint4*>(row + (j ^ (lane & 7)) * 16) =
+                                make_uint4(gemm::pack_bf16x2(half[at], half[at + 1]),
+                                           gemm::pack_bf16x2(half[at + 2], half[at + 3]),
+                                           gemm::pack_bf16x2(half[at + 4], half[at + 5]),
+                                           gemm::pack_bf16x2(half[at + 6], half[at + 7]));
+                        }
+                        send(w.b0 + c);
                     }
-                    ptx::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0 && n0 < p.n) {
-                        const int col = w.b0 + (second ? c - 32 : c);
-                        if (p.accumulate)
-                            ptx::tma_add_3d(&map_c, buf, col, n0, w.e);
-                        else
-                            ptx::tma_store_3d(&map_c, buf, col, n0, w.e);
-                        ptx::bulk_commit_group();
-                    }
-                    ++stored;
                 }
+            }
+            if (computed) {
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.tmem_empty[acc]), 0));
             }
         }
         if constexpr (L::kGrad) {
             if (lane == 0) ptx::bulk_wait_group_read<0>();  // shared memory outlives the stores' reads of it
         }
         __syncwarp();
-    } else if (L::kMx && warp == 10) {
+    } else if (L::kMx && warp == kExtraWarp + 4) {
         // ------------------------------------------------- scales into TMEM
         // Per stage two words of 4 columns for the weight rows, two of 8 for
         // the tokens.  Its own thread issues the copies and a commit tells the
@@ -428,7 +451,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
             Ring<S> ring;
             bool ok = true;
             for (int t = first_tile; t < tiles && ok; t += tile_step) {
-                const Tile w = tile_at<KIND>(table, p, t);
+                const Tile w = tile_at<KIND>(table, p, t, group);
                 for (int kb = 0; kb < w.blocks; ++kb) {
                     if (!ptx::mbar_wait_cluster(&bar.full[ring.stage], ring.phase, p.limit_ns, abort)) {
                         record_failure(p.status, abort, kRoleMma);
@@ -463,7 +486,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
         // in shared memory.  Scales come four stages at a time, two 16-byte
         // loads a row, and the next four stages' are under way while these are
         // handed out.
-        const int i = (warp - 6) * 8 + lane / 4 + lane % 4 * 32;
+        const int i = (warp - kExtraWarp) * 8 + lane / 4 + lane % 4 * 32;
         const int blocks32 = p.k / 32;
         Ring<S> ring;
         bool ok = true;
@@ -471,7 +494,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
         Tile w = {};
         const uint8_t* rows[3] = {};
         auto start_tile = [&] {
-            w = tile_at<KIND>(table, p, t);
+            w = tile_at<KIND>(table, p, t, group);
             const int n = w.n0 + rank * 128 + i;
             rows[0] = n < p.n ? p.w_scales + w.e * p.ws_stride + n * p.ldws : nullptr;
             for (int j = 0; j < 2; ++j)
@@ -533,7 +556,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
         Ring<S> ring;
         uint32_t landed_phase = 0;  // a bit per stage
         for (int t = first_tile; t < tiles; t += tile_step) {
-            const Tile w = tile_at<KIND>(table, p, t);
+            const Tile w = tile_at<KIND>(table, p, t, group);
             for (int kb = 0; kb < w.blocks - 1; ++kb) ring.next();
             if (w.blocks == 0) continue;
             if (w.tail != 0) {

@@ -49,8 +49,9 @@ __global__ void __launch_bounds__(kThreads) grouped_forward_simt(ForwardArgs p) 
         build_group_table(table, p.ends, p.rows, [&](int rows) { return (rows + kTile - 1) / kTile * tiles_n; });
     __syncthreads();
     auto* y = static_cast<__nv_bfloat16*>(p.y);
+    int group = 0;
     for (int t = blockIdx.x; t < table.tiles(); t += gridDim.x) {
-        const int e = group_of_tile(table, t);
+        const int e = group_of_tile(table, t, group);
         const int in_group = t - table.tile[e];
         const int64_t row0 = table.row[e] + in_group / tiles_n * kTile;
         const int col0 = in_group % tiles_n * kTile;

@@ -70,9 +70,10 @@ struct Tile {
 };
 
 template <Kind KIND>
-__device__ __forceinline__ Tile tile_at(const GroupTable& table, const SplitParams& p, int t, int rank, int splits) {
+__device__ __forceinline__ Tile tile_at(const GroupTable& table, const SplitParams& p, int t, int rank, int splits,
+                                        int& group) {
     Tile out;
-    out.e = group_of_tile(table, t);
+    out.e = group_of_tile(table, t, group);
     const int in_group = t - table.tile[out.e];
     const int first = table.row[out.e], rows = table.row[out.e + 1] - first;
     const int tiles_t = (rows + kMaxWidth - 1) / kMaxWidth;
@@ -155,6 +156,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
     ptx::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int tiles = table.tiles();
+    int group = 0;  // the last tile's
 
     if (warp == 0) {
         // ------------------------------------------------------------ producer
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
             uint32_t issued = 0, issued_phase = 0;
             bool ok = true;
             for (int t = first_tile; t < tiles && ok; t += tile_step) {
-                const Tile w = tile_at<KIND>(table, p, t, rank, splits);
+                const Tile w = tile_at<KIND>(table, p, t, rank, splits, group);
                 const CUtensorMap* mb = w.width > 32 ? &map_b64 : w.width > 16 ? &map_b32 : &map_b16;
                 const int box_rows = w.width > 32 ? 64 : w.width > 16 ? 32 : 16;
                 for (int kb = w.kb0; kb < w.kb1; ++kb) {
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
             int local = 0;
             bool ok = true;
             for (int t = first_tile; t < tiles && ok; t += tile_step) {
-                const Tile w = tile_at<KIND>(table, p, t, rank, splits);
+                const Tile w = tile_at<KIND>(table, p, t, rank, splits, group);
                 if (w.kb0 == w.kb1) continue;
                 const int acc = local & 1;
                 if (!ptx::mbar_wait(&tmem_empty[acc], ((local >> 1) & 1) ^ 1u, p.limit_ns, abort)) {
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
         int local = 0, seen = 0;
         bool ok = true;
         for (int t = first_tile; t < tiles && ok; t += tile_step, ++seen) {
-            const Tile w = tile_at<KIND>(table, p, t, rank, splits);
+            const Tile w = tile_at<KIND>(table, p, t, rank, splits, group);
             const bool computed = w.kb0 != w.kb1;
             const int acc = local & 1;
             if (computed) {
@@ -336,7 +338,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
             Ring<S> ring;
             bool ok = true;
             for (int t = first_tile; t < tiles && ok; t += tile_step) {
-                const Tile w = tile_at<KIND>(table, p, t, rank, splits);
+                const Tile w = tile_at<KIND>(table, p, t, rank, splits, group);
                 for (int kb = w.kb0; kb < w.kb1; ++kb) {
                     if (!ptx::mbar_wait(&full[ring.stage], ring.phase, p.limit_ns, abort)) {
                         record_failure(p.status, abort, kRoleMma);
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
         // CTA's first stage is: loads are aligned.
         auto start_tile = [&] {
             for (; t < tiles; t += tile_step) {
-                w = tile_at<KIND>(table, p, t, rank, splits);
+                w = tile_at<KIND>(table, p, t, rank, splits, group);
                 if (w.kb0 < w.kb1) break;
             }
             if (t >= tiles) return;

@@ -82,16 +82,42 @@ __device__ __forceinline__ void load_scales(const uint8_t* row, int first, int b
     out[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-// Writes a 32-token chunk of an accumulator whose lanes are output columns:
-// lane l holds column col0 + l of tokens 0..31 in r[].  The values turn round
-// in a 32 x 64-byte staging buffer of the warp's own, so that four lanes write
-// 64 consecutive bytes of one token's row.
+// 32 TMEM lanes x 32 columns in the registers of 8 x 8 matrices: after it, r[16
+// h + 4 t + 2 g + i] is lane 16 h + 8 g + l / 4, column 8 t + 2 (l % 4) + i, for
+// thread l of the warp.
+__device__ __forceinline__ void load_rows_of_8(uint32_t taddr, uint32_t (&r)[32]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t* q = r + 16 * h;
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
+              "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15])
+            : "r"(taddr + (static_cast<uint32_t>(16 * h) << 16)));
+    }
+    ptx::tmem_wait_ld();
+}
+
+// Writes a 32-token chunk of an accumulator whose lanes are output columns
+// (from load_rows_of_8): lane l is column col0 + l of tokens 0..31.  The values
+// turn round in a 32 x 64-byte staging buffer of the warp's own, four 8 x 8
+// matrices at a time, so that four threads write 64 consecutive bytes of one
+// token's row.  Chunk j of token t's 64 bytes stands at j ^ (t / 2) % 4: no two
+// rows of a matrix share banks.
 __device__ __forceinline__ void store_transposed(const uint32_t (&r)[32], uint8_t* staging, __nv_bfloat16* y,
                                                  int64_t ldy, int tokens, int col0, int n, bool vec, int lane) {
     __syncwarp();  // the chunk before has been read
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-        *reinterpret_cast<__nv_bfloat16*>(staging + j * 64 + lane * 2) = __float2bfloat16_rn(__uint_as_float(r[j]));
+    for (int t = 0; t < 4; ++t) {
+        const int token = 8 * t + lane % 8;
+        const uint32_t at = ptx::smem_addr(staging + token * 64 + ((lane / 8) ^ (token / 2 % 4)) * 16);
+        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at),
+                     "r"(gemm::pack_bf16x2(r[4 * t], r[4 * t + 1])), "r"(gemm::pack_bf16x2(r[4 * t + 2], r[4 * t + 3])),
+                     "r"(gemm::pack_bf16x2(r[16 + 4 * t], r[16 + 4 * t + 1])),
+                     "r"(gemm::pack_bf16x2(r[16 + 4 * t + 2], r[16 + 4 * t + 3]))
+                     : "memory");
+    }
     __syncwarp();
     const int col = col0 + lane % 4 * 8;
 #pragma unroll
@@ -99,7 +125,7 @@ __device__ __forceinline__ void store_transposed(const uint32_t (&r)[32], uint8_
         const int j = i * 8 + lane / 4;
         if (j >= tokens || col >= n) continue;
         __nv_bfloat16* dst = y + j * ldy + col;
-        const auto* src = reinterpret_cast<const __nv_bfloat16*>(staging + j * 64) + lane % 4 * 8;
+        const auto* src = reinterpret_cast<const __nv_bfloat16*>(staging + j * 64 + (lane % 4 ^ (j / 2 % 4)) * 16);
         if (vec && col + 8 <= n) {
             *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
         } else {
