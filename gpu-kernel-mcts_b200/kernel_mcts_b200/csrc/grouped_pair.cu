@@ -67,6 +67,7 @@ struct PairParams {
     bool vec;           // y rows take 16-byte stores
     bool zero_rest;
     bool fp32, accumulate;  // gradient
+    bool stream_out;        // gradient: larger than half of L2
     const uint8_t* x_scales;
     int64_t ldxs;
     const uint8_t* w_scales;
@@ -375,7 +376,10 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                 // TMA, which clips them at the group's own edges: columns of a
                 // last chunk past the width are past the row's end too.
                 // (64-byte rows of BF16 took 311 us for 16 groups of 512 rows,
-                // 4096 x 4096.)
+                // 4096 x 4096.)  A gradient that L2 cannot hold leaves it
+                // first, in about the order it came (from 64 rows a group 112
+                // us without, 91 with).
+                const uint64_t policy = p.stream_out ? ptx::policy_evict_first() : ptx::policy_evict_normal();
                 auto send = [&](int col) {
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                         if (p.accumulate)
                             ptx::tma_add_3d(&map_c, staging, col, n0, w.e);
                         else
-                            ptx::tma_store_3d(&map_c, staging, col, n0, w.e);
+                            ptx::tma_store_3d_hint(&map_c, staging, col, n0, w.e, policy);
                         ptx::bulk_commit_group();
                     }
                 };
@@ -695,6 +699,7 @@ int launch_wgrad_pair(const WgradArgs& g, uint64_t limit_ns, cudaStream_t stream
                         strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
             return KMCTS_ENOTSUP;
     }
+    p.stream_out = static_cast<int64_t>(g.groups) * g.n * g.k * (g.fp32 ? 4 : 2) > 63LL << 20;  // L2 is 126 MB
     const int64_t tiles = static_cast<int64_t>(g.groups) * ((g.n + 255) / 256) * ((g.k + 255) / 256);
     if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;
     return launch<Kind::kWgrad>(a, b, c, p, tiles, stream);

@@ -28,12 +28,13 @@ __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* m
         : "memory");
 }
 
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int32_t c0, int32_t c1,
-                                             int32_t c2) {
+// With an L2 cache policy (from createpolicy).
+__device__ __forceinline__ void tma_store_3d_hint(const CUtensorMap* map, const void* src, int32_t c0, int32_t c1,
+                                                  int32_t c2, uint64_t policy) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+        "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group.L2::cache_hint [%0, {%2, %3, %4}], [%1], %5;" ::"l"(
             reinterpret_cast<uint64_t>(map)),
-        "r"(smem_addr(src)), "r"(c0), "r"(c1), "r"(c2)
+        "r"(smem_addr(src)), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
         : "memory");
 }
 
