@@ -42,6 +42,13 @@ struct WgradArgs {
     int groups, rows, n, k;
 };
 
+// Fills in a launch attribute: the grid's blocks may start before the grids
+// ahead of it in the stream have finished; its kernel waits for them itself.
+inline void allow_early_start(cudaLaunchAttribute* attr) {
+    attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr->val.programmaticStreamSerializationAllowed = 1;
+}
+
 enum class Operand { kBf16Col, kBf16Row, kMxfp4 };
 
 // The tensor-core launchers return KMCTS_ENOTSUP, having launched nothing, for

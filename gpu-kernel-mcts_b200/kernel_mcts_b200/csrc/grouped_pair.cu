@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
     const bool leader = rank == 0;
     const int first_tile = blockIdx.x / 2, tile_step = gridDim.x / 2;
 
+    ptx::let_next_grid_start();
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             // MXFP4: besides the leader's byte count, four scale warps of each CTA.
@@ -183,6 +184,8 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
         ptx::tmem_alloc_pair(tmem_slot, 512);
         ptx::tmem_relinquish_pair();
     }
+    // Up to here the launch overlaps the end of the grid before.
+    ptx::wait_for_earlier_grids();
     if (warp == 2) {
         const int tiles_a = (p.n + 255) / 256;
         if constexpr (L::kGrad) {
@@ -633,17 +636,18 @@ int launch(const CUtensorMap& a, const CUtensorMap (&b)[3], const CUtensorMap& c
     }
     const int64_t pairs = multiprocessor_count() / 2;
     cudaLaunchConfig_t config = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    allow_early_start(&attr[1]);
     config.gridDim = dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)), 1, 1);
     config.blockDim = dim3(L::kThreads, 1, 1);
     config.dynamicSmemBytes = L::smem_bytes(p.groups);
     config.stream = stream;
     config.attrs = attr;
-    config.numAttrs = 1;
+    config.numAttrs = 2;
     const cudaError_t err = cudaLaunchKernelEx(&config, grouped_pair_kernel<KIND>, a, b[0], b[1], b[2], c, p);
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return err == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;

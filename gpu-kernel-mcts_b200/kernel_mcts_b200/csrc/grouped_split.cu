@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
     const int splits = static_cast<int>(ptx::cluster_nctarank());
     const int first_tile = blockIdx.x / splits, tile_step = gridDim.x / splits;
 
+    ptx::let_next_grid_start();
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             ptx::mbar_init(&full[s], L::kMx ? 5 : 1);  // MXFP4: the byte count and four scale warps
@@ -144,6 +145,8 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
         ptx::tmem_alloc(tmem_slot, L::kTmemCols);
         ptx::tmem_relinquish();
     }
+    // Up to here the launch overlaps the end of the grid before.
+    ptx::wait_for_earlier_grids();
     if (warp == 2) {
         const int tiles_n = (p.n + 127) / 128;
         build_group_table(table, p.ends, p.rows,
@@ -484,16 +487,17 @@ int launch(const CUtensorMap& a, const CUtensorMap (&b)[3], const SplitParams& p
     const int64_t clusters = resident_clusters<KIND>(device, splits);
     if (clusters <= 0) return KMCTS_EGEMM;
     cudaLaunchConfig_t config = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = splits;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    allow_early_start(&attr[1]);
     config.gridDim = dim3(static_cast<unsigned>(splits * (tiles < clusters ? tiles : clusters)), 1, 1);
     config.blockDim = dim3(L::kThreads, 1, 1);
     config.dynamicSmemBytes = L::smem_bytes(p.groups);
     config.stream = stream;
     config.attrs = attr;
-    config.numAttrs = 1;
+    config.numAttrs = 2;
     const cudaError_t err = cudaLaunchKernelEx(&config, grouped_split_kernel<KIND>, a, b[0], b[1], b[2], p);
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return err == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;

@@ -9,6 +9,7 @@
 // block a thread took 128 us (128 bytes a lane outrun L1), half a block 91 us.
 // Restoring, a thread writes 8 elements at a time, four times (58 us).
 #include "grouped_common.cuh"
+#include "ptx_grouped.cuh"
 
 namespace kmcts {
 namespace {
@@ -118,6 +119,8 @@ __global__ void __launch_bounds__(kThreads)
     mxfp4_quantize_kernel(const typename Element<TYPE>::type* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
                           int64_t ldc, uint8_t* __restrict__ scales, int64_t lds, int64_t rows, unsigned per_row,
                           unsigned rows_per_block) {
+    ptx::let_next_grid_start();
+    ptx::wait_for_earlier_grids();
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
     const unsigned here = static_cast<unsigned>(min(static_cast<int64_t>(rows_per_block), rows - row0));
     const unsigned total = here * per_row;
@@ -172,6 +175,8 @@ __global__ void __launch_bounds__(kThreads)
     mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
                             int64_t lds, typename Element<TYPE>::type* __restrict__ out, int64_t ldo, int64_t rows,
                             unsigned per_row, unsigned rows_per_block) {
+    ptx::let_next_grid_start();
+    ptx::wait_for_earlier_grids();
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
     const unsigned here = static_cast<unsigned>(min(static_cast<int64_t>(rows_per_block), rows - row0));
     const unsigned total = here * per_row;
@@ -230,6 +235,21 @@ unsigned rows_per_block(int64_t rows, unsigned per_row, int each) {
     return fit < 1 ? 1 : fit;
 }
 
+template <typename... Params, typename... Args>
+int launch(void (*kernel)(Params...), int64_t blocks, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute attr[1];
+    grouped::allow_early_start(&attr[0]);
+    config.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+    config.blockDim = dim3(kThreads, 1, 1);
+    config.stream = stream;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return err == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
+}
+
 template <int TYPE>
 int quantize(const void* X, int64_t ldx, uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds, int64_t rows,
              int K, cudaStream_t stream) {
@@ -237,15 +257,9 @@ int quantize(const void* X, int64_t ldx, uint8_t* codes, int64_t ldc, uint8_t* s
     const unsigned per_row = K / 32 * kSharing<TYPE>, per_block = rows_per_block(rows, per_row, 1);
     const int64_t blocks = (rows + per_block - 1) / per_block;
     if (blocks > 0x7fffffff) return KMCTS_EINVAL;
-    auto* x = static_cast<const T*>(X);
-    if (aligned(X, ldx * sizeof(T), 16) && aligned(codes, ldc, 16))
-        mxfp4_quantize_kernel<TYPE, true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-            x, ldx, codes, ldc, scales, lds, rows, per_row, per_block);
-    else
-        mxfp4_quantize_kernel<TYPE, false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-            x, ldx, codes, ldc, scales, lds, rows, per_row, per_block);
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    return cudaGetLastError() == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
+    const bool vec = aligned(X, ldx * sizeof(T), 16) && aligned(codes, ldc, 16);
+    return launch(vec ? mxfp4_quantize_kernel<TYPE, true> : mxfp4_quantize_kernel<TYPE, false>, blocks, stream,
+                  static_cast<const T*>(X), ldx, codes, ldc, scales, lds, rows, per_row, per_block);
 }
 
 template <int TYPE>
@@ -255,15 +269,9 @@ int dequantize(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t
     const unsigned per_row = K / kChunk, per_block = rows_per_block(rows, per_row, kBatch);
     const int64_t blocks = (rows + per_block - 1) / per_block;
     if (blocks > 0x7fffffff) return KMCTS_EINVAL;
-    auto* o = static_cast<T*>(out);
-    if (aligned(out, ldo * sizeof(T), 16) && aligned(codes, ldc, 4))
-        mxfp4_dequantize_kernel<TYPE, true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-            codes, ldc, scales, lds, o, ldo, rows, per_row, per_block);
-    else
-        mxfp4_dequantize_kernel<TYPE, false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-            codes, ldc, scales, lds, o, ldo, rows, per_row, per_block);
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    return cudaGetLastError() == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
+    const bool vec = aligned(out, ldo * sizeof(T), 16) && aligned(codes, ldc, 4);
+    return launch(vec ? mxfp4_dequantize_kernel<TYPE, true> : mxfp4_dequantize_kernel<TYPE, false>, blocks, stream,
+                  codes, ldc, scales, lds, static_cast<T*>(out), ldo, rows, per_row, per_block);
 }
 
 }  // namespace

@@ -8,6 +8,15 @@
 namespace kmcts {
 namespace ptx {
 
+// Programmatic dependent launch.  wait_for_earlier_grids returns once the
+// grids before this one in the stream have finished and their writes are
+// visible (at once where the launch did not ask for overlap); every access of
+// global memory comes after it.  let_next_grid_start allows the next grid's
+// blocks onto SMs that have room for them, up to their own wait.
+__device__ __forceinline__ void wait_for_earlier_grids() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__device__ __forceinline__ void let_next_grid_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // With an L2 cache policy (from createpolicy).
 __device__ __forceinline__ void tma_load_3d_hint(void* dst, const CUtensorMap* map, uint64_t* bar, int32_t c0,
                                                  int32_t c1, int32_t c2, uint64_t policy) {

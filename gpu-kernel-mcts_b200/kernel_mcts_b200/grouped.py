@@ -155,8 +155,9 @@ class _GroupedLinear(torch.autograd.Function):
         return grouped_gemm(x, w, ends)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():  # create_graph: the gradients below would not be part of it
+            raise RuntimeError("grouped_linear is differentiable once")
         x, w, ends = ctx.saved_tensors
         dy = _strided_rows(dy)
         dx = grouped_gemm(dy, w, ends, w_layout="row") if ctx.needs_input_grad[0] else None

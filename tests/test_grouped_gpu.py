@@ -266,6 +266,39 @@ def test_only_the_gradients_asked_for_are_computed(cuda_device):
     assert _native.launch_count() == before + 1 and w.grad is not None
 
 
+def test_second_derivatives_are_refused(cuda_device):
+    x, w = integers(8, 16, seed=1).requires_grad_(), integers(1, 8, 16, seed=2)
+    y = grouped.grouped_linear(x, w, ends_of([8]))
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_calls_in_a_row_see_each_other(cuda_device):
+    """A chain of calls that each read what the one before wrote, long enough
+    that launches overlap: directly and as a graph."""
+    counts, n = [3, 60, 1], 256
+    w = torch.zeros(3, n, n, dtype=torch.bfloat16, device="cuda")
+    w[:, torch.arange(n), torch.arange(n).roll(1)] = 1  # y[:, j] = x[:, j - 1]
+    ends, x = ends_of(counts), integers(64, n, seed=1)
+    buffers = [torch.empty_like(x) for _ in range(2)]
+
+    def chain():
+        y = x
+        for i in range(40):
+            kernel = ("pair", "split")[i // 2 % 2]
+            y = grouped.grouped_gemm(y, w, ends, buffers[i % 2], kernel=kernel)
+
+    chain()
+    assert torch.equal(buffers[1], x.roll(40, 1))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain()
+    x.copy_(integers(64, n, seed=2))
+    graph.replay()
+    graph.replay()
+    assert torch.equal(buffers[1], x.roll(40, 1))
+
+
 def test_side_stream_and_graph_replay(cuda_device):
     counts, n, k = [40, 3, 90], 128, 256
     x, w = integers(sum(counts), k, seed=1), integers(3, n, k, seed=2)
