@@ -11,6 +11,7 @@ import contextlib
 import torch
 
 MAX_GROUPS = 1024
+MAX_SIZE = 2 ** 31 - 2 ** 10  # rows, N and K are 32-bit numbers in the kernels, with room to round up
 
 _current_device = torch.cuda.current_device
 
@@ -61,6 +62,11 @@ def check_groups(ends: torch.Tensor, index: int) -> int:
     if not 1 <= groups <= MAX_GROUPS:
         raise ValueError(f"there must be 1 to {MAX_GROUPS} groups, got {groups}")
     return groups
+
+
+def check_sizes(*sizes: int) -> None:
+    if max(sizes) > MAX_SIZE:
+        raise ValueError(f"sizes must be at most {MAX_SIZE}, got {sizes}")
 
 
 def status_pointer(status: torch.Tensor | None, index: int) -> int | None:

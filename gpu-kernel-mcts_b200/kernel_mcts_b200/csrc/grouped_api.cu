@@ -66,8 +66,12 @@ using namespace kmcts::grouped;
 
 namespace {
 
-bool bad_groups(const int32_t* ends, int groups, int rows, int n, int k) {
-    return rows < 0 || n < 0 || k < 0 || groups < 1 || groups > KMCTS_MAX_GROUPS || !ends;
+// Sizes leave room to round up to whole tiles.
+constexpr int kMaxSize = 0x7fffffff - 1023;
+
+bool bad_sizes(int groups, int rows, int n, int k) {
+    return rows < 0 || n < 0 || k < 0 || rows > kMaxSize || n > kMaxSize || k > kMaxSize || groups < 1 ||
+           groups > KMCTS_MAX_GROUPS;
 }
 
 // Whether the few-rows kernel should take a product, and how many CTAs share
@@ -120,7 +124,7 @@ extern "C" {
 int kmcts_bf16_grouped_gemm(const void* X, int64_t ldx, const void* W, int64_t w_stride, int64_t ldw, int w_layout,
                             void* Y, int64_t ldy, const int32_t* ends, int groups, int rows, int N, int K, int flags,
                             int kernel, void* stream, int* device_status) {
-    if (bad_groups(ends, groups, rows, N, K)) return KMCTS_EINVAL;
+    if (bad_sizes(groups, rows, N, K) || !ends) return KMCTS_EINVAL;
     if (w_layout != KMCTS_B_COL && w_layout != KMCTS_B_ROW) return KMCTS_EINVAL;
     if (rows > 0 && N > 0 && (!Y || ldy < N || (K > 0 && (!X || !W || ldx < K)))) return KMCTS_EINVAL;
     if (ldw < (w_layout == KMCTS_B_COL ? K : N) || w_stride < 0) return KMCTS_EINVAL;
@@ -137,7 +141,7 @@ int kmcts_bf16_grouped_gemm(const void* X, int64_t ldx, const void* W, int64_t w
 int kmcts_bf16_grouped_wgrad(const void* dY, int64_t lddy, const void* X, int64_t ldx, void* dW, int64_t dw_stride,
                              int64_t lddw, int dw_type, int accumulate, const int32_t* ends, int groups, int rows,
                              int N, int K, int kernel, void* stream, int* device_status) {
-    if (bad_groups(ends, groups, rows, N, K)) return KMCTS_EINVAL;
+    if (bad_sizes(groups, rows, N, K) || !ends) return KMCTS_EINVAL;
     if (dw_type != KMCTS_TYPE_BF16 && dw_type != KMCTS_TYPE_FP32) return KMCTS_EINVAL;
     if (accumulate && dw_type != KMCTS_TYPE_FP32) return KMCTS_EINVAL;
     if (N == 0 || K == 0) return KMCTS_OK;
@@ -163,8 +167,7 @@ int kmcts_mxfp4_gemm(const void* A, int64_t lda, const void* A_scales, int64_t l
                      int64_t ldb, const void* B_scales, int64_t bs_stride, int64_t ldbs, void* Y, int64_t ldy,
                      const int32_t* ends, int groups, int rows, int N, int K, int flags, int kernel, void* stream,
                      int* device_status) {
-    if (rows < 0 || N < 0 || K < 0 || K % 32 != 0 || groups < 1 || groups > KMCTS_MAX_GROUPS) return KMCTS_EINVAL;
-    if (!ends && groups != 1) return KMCTS_EINVAL;
+    if (bad_sizes(groups, rows, N, K) || K % 32 != 0 || (!ends && groups != 1)) return KMCTS_EINVAL;
     if (rows > 0 && N > 0 && (!Y || ldy < N)) return KMCTS_EINVAL;
     if (rows > 0 && N > 0 && K > 0 && (!A || !A_scales || !B || !B_scales)) return KMCTS_EINVAL;
     if (lda < K / 2 || ldb < K / 2 || ldas < K / 32 || ldbs < K / 32 || b_stride < 0 || bs_stride < 0)

@@ -138,6 +138,7 @@ unsigned grid_for(int64_t tiles) {
 int launch_forward_simt(const ForwardArgs& a, Operand kind, cudaStream_t stream) {
     // Every group may end in a partly filled tile.
     const int64_t tiles = (static_cast<int64_t>((a.rows + kTile - 1) / kTile) + a.groups) * ((a.n + kTile - 1) / kTile);
+    if (tiles > 0x7fffffff) return KMCTS_ENOTSUP;
     const unsigned grid = grid_for(tiles);
     switch (kind) {
         case Operand::kBf16Col:
@@ -156,6 +157,7 @@ int launch_forward_simt(const ForwardArgs& a, Operand kind, cudaStream_t stream)
 
 int launch_wgrad_simt(const WgradArgs& a, cudaStream_t stream) {
     const int64_t tiles = static_cast<int64_t>(a.groups) * ((a.n + kTile - 1) / kTile) * ((a.k + kTile - 1) / kTile);
+    if (tiles > 0x7fffffff) return KMCTS_ENOTSUP;
     grouped_wgrad_simt<<<grid_for(tiles), kThreads, table_bytes(a.groups), stream>>>(a);
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return cudaGetLastError() == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;

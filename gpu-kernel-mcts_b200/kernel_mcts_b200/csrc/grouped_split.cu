@@ -500,7 +500,9 @@ int launch(const CUtensorMap& a, const CUtensorMap (&b)[3], const SplitParams& p
     config.numAttrs = 2;
     const cudaError_t err = cudaLaunchKernelEx(&config, grouped_split_kernel<KIND>, a, b[0], b[1], b[2], p);
     g_launches.fetch_add(1, std::memory_order_relaxed);
-    return err == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
+    if (err == cudaSuccess) return KMCTS_OK;
+    cudaGetLastError();  // reported here, not by the caller's next call
+    return KMCTS_EGEMM;
 }
 
 }  // namespace

@@ -247,7 +247,9 @@ int launch(void (*kernel)(Params...), int64_t blocks, cudaStream_t stream, Args.
     config.numAttrs = 1;
     const cudaError_t err = cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
     g_launches.fetch_add(1, std::memory_order_relaxed);
-    return err == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
+    if (err == cudaSuccess) return KMCTS_OK;
+    cudaGetLastError();  // reported here, not by the caller's next call
+    return KMCTS_EGEMM;
 }
 
 template <int TYPE>

@@ -67,6 +67,7 @@ def grouped_gemm(
         raise ValueError(f"inner dimensions differ: x has K={k}, w has K={kw}")
     if w_shape[0] != groups:
         raise ValueError(f"w holds {w_shape[0]} groups, ends {groups}")
+    _launch.check_sizes(rows, n, k)
     status_ptr = _launch.status_pointer(status, device)
     kernel_id = kernel_code(kernel)
     caller = _launch.caller_stream(device, stream)
@@ -112,6 +113,7 @@ def grouped_gemm_wgrad(
     groups = _launch.check_groups(ends, device)
     if x_rows != rows:
         raise ValueError(f"dy has {rows} rows, x {x_rows}")
+    _launch.check_sizes(rows, n, k)
     if dtype is None:
         dtype = out.dtype if out is not None else torch.bfloat16
     if dtype not in _GRADIENT_TYPES:

@@ -82,6 +82,7 @@ def mxfp4_quantize(
     flat = _rows("x", x)
     device = x.get_device()
     (rows, k), _, ldx = _launch.rows_of("x", flat, 2, _TYPE_TUPLE, device, BLOCK)
+    _launch.check_sizes(k)
     caller = _launch.caller_stream(device, stream)
     with _launch.on_device(device, stream):
         if out is None:
@@ -117,6 +118,7 @@ def mxfp4_dequantize(
     if q.scales.shape[:-1] != q.codes.shape[:-1]:
         raise ValueError(f"q scales must go with codes of shape {tuple(q.codes.shape)}, got {tuple(q.scales.shape)}")
     k = 2 * half
+    _launch.check_sizes(k)
     if dtype is None:
         dtype = out.dtype if out is not None else torch.bfloat16
     if dtype not in _TYPES:
@@ -161,6 +163,7 @@ def mxfp4_gemm(
     if b_shape[-1] != half:
         raise ValueError(f"inner dimensions differ: a has K={2 * half}, b has K={2 * b_shape[-1]}")
     k, n = 2 * half, b_shape[-2]
+    _launch.check_sizes(rows, n, k)
     groups, ends_ptr, b_stride, bs_stride = 1, None, 0, 0
     if ends is not None:
         groups, ends_ptr = _launch.check_groups(ends, device), ends.data_ptr()
