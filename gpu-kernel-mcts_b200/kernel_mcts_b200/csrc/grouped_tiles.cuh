@@ -119,6 +119,16 @@ __device__ __forceinline__ void store_transposed(const uint32_t (&r)[32], uint8_
                      : "memory");
     }
     __syncwarp();
+    if (!vec) {
+        // Rows at any alignment: 32 threads write 64 consecutive bytes, two
+        // each (16 experts, 8192 rows, 4095 x 4096: 307 us with eight
+        // two-byte stores for each 16 bytes, 231 so).
+        if (col0 + lane < n)
+            for (int j = 0; j < min(tokens, 32); ++j)
+                y[j * ldy + col0 + lane] = *reinterpret_cast<const __nv_bfloat16*>(
+                    staging + j * 64 + ((lane / 8) ^ (j / 2 % 4)) * 16 + lane % 8 * 2);
+        return;
+    }
     const int col = col0 + lane % 4 * 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -126,7 +136,7 @@ __device__ __forceinline__ void store_transposed(const uint32_t (&r)[32], uint8_
         if (j >= tokens || col >= n) continue;
         __nv_bfloat16* dst = y + j * ldy + col;
         const auto* src = reinterpret_cast<const __nv_bfloat16*>(staging + j * 64 + (lane % 4 ^ (j / 2 % 4)) * 16);
-        if (vec && col + 8 <= n) {
+        if (col + 8 <= n) {
             *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
         } else {
             for (int b = 0; b < 8 && col + b < n; ++b) dst[b] = src[b];
