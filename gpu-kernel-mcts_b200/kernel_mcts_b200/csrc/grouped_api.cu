@@ -52,10 +52,11 @@ bool encode_forward_maps(const ForwardArgs& f, Operand operand, CUtensorMap* w, 
     return true;
 }
 
-int scale_alignment(const ForwardArgs& f) {
-    const uintptr_t starts = reinterpret_cast<uintptr_t>(f.x_scales) | reinterpret_cast<uintptr_t>(f.w_scales) |
-                             static_cast<uintptr_t>(f.ldxs | f.ldws | f.ws_stride);
-    return starts % 16 == 0 ? 16 : starts % 8 == 0 ? 8 : 1;
+void scale_spans(const ForwardArgs& f, ScaleSpan* x, ScaleSpan* w) {
+    *x = *w = {nullptr, nullptr};
+    if (f.x_scales == nullptr) return;
+    *x = {f.x_scales, f.x_scales + (f.rows - 1) * f.ldxs + f.k / 32};
+    *w = {f.w_scales, f.w_scales + (f.groups - 1) * f.ws_stride + (f.n - 1) * f.ldws + f.k / 32};
 }
 
 }  // namespace grouped

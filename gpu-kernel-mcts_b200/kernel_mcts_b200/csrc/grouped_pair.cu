@@ -78,7 +78,7 @@ struct PairParams {
     int64_t ldxs;
     const uint8_t* w_scales;
     int64_t ws_stride, ldws;
-    int scale_align;  // bytes that every row of scales starts at a multiple of
+    ScaleSpan x_span, w_span;
     uint64_t limit_ns;
     int* status;
 };
@@ -500,9 +500,9 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
         // Thread i holds one of this CTA's 128 weight rows and two of the
         // tile's tokens (both CTAs need every token's scales): rows l / 4 + 32
         // (l % 4) + 8 warps for lane l, so that a warp's words lie side by side
-        // in shared memory.  Scales come four stages at a time, two 16-byte
-        // loads a row, and the next four stages' are under way while these are
-        // handed out.
+        // in shared memory.  Scales come four stages at a time, two or three
+        // 16-byte loads a row, and the next four stages' are under way while
+        // these are handed out.
         const int i = (warp - kExtraWarp) * 8 + lane / 4 + lane % 4 * 32;
         const int blocks32 = p.k / 32;
         Ring<S> ring;
@@ -517,19 +517,19 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
             for (int j = 0; j < 2; ++j)
                 rows[1 + j] = i + 128 * j < w.valid ? p.x_scales + (static_cast<int64_t>(w.b0) + i + 128 * j) * p.ldxs : nullptr;
         };
-        uint4 v[3][2], next[3][2];  // 32 bytes of each row: stages kb0 .. kb0 + 3
-        auto load = [&](uint4 (&to)[3][2]) {
+        uint4 words[3][3], v[3][2];  // of each row: 32 scales for stages kb0 .. kb0 + 3, and the last four's
+        auto load = [&] {
 #pragma unroll
-            for (int j = 0; j < 3; ++j) {
-                to[j][0] = to[j][1] = make_uint4(0, 0, 0, 0);
-                if (rows[j]) load_scales(rows[j], kb0 * 8, blocks32, p.scale_align, to[j]);
-            }
+            for (int j = 0; j < 3; ++j)
+                load_scale_words(rows[j], kb0 * 8, blocks32, j == 0 ? p.w_span : p.x_span, words[j]);
         };
         if (t < tiles) {
             start_tile();
-            load(v);
+            load();
         }
         while (t < tiles && ok) {
+#pragma unroll
+            for (int j = 0; j < 3; ++j) align_scales(rows[j], kb0 * 8, blocks32, words[j], v[j]);
             const int here = min(4, w.blocks - kb0);
             kb0 += 4;
             if (kb0 >= w.blocks) {
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                 t += tile_step;
                 if (t < tiles) start_tile();
             }
-            if (t < tiles) load(next);
+            if (t < tiles) load();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 if (q >= here || !ok) break;
@@ -564,8 +564,6 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                 if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_addr(&bar.full[ring.stage]), 0));
                 ring.next();
             }
-#pragma unroll
-            for (int j = 0; j < 3; ++j) v[j][0] = next[j][0], v[j][1] = next[j][1];
         }
         __syncwarp();
     } else if constexpr (L::kGrad) {
@@ -675,7 +673,7 @@ int launch_forward_pair(const ForwardArgs& f, Operand operand, uint64_t limit_ns
     p.zero_rest = f.zero_rest;
     p.x_scales = f.x_scales, p.ldxs = f.ldxs;
     p.w_scales = f.w_scales, p.ws_stride = f.ws_stride, p.ldws = f.ldws;
-    p.scale_align = scale_alignment(f);
+    scale_spans(f, &p.x_span, &p.w_span);
     p.limit_ns = limit_ns, p.status = status;
     const bool mx = operand == Operand::kMxfp4;
     const uint32_t box_rows[3] = {mx ? 96u : 128u, 64, 32};

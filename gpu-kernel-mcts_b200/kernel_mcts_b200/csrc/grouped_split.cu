@@ -58,7 +58,7 @@ struct SplitParams {
     int64_t ldxs;
     const uint8_t* w_scales;
     int64_t ws_stride, ldws;
-    int scale_align;
+    ScaleSpan x_span, w_span;
     uint64_t limit_ns;
     int* status;
 };
@@ -385,24 +385,24 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
             rows[0] = n < p.n ? p.w_scales + w.e * p.ws_stride + n * p.ldws : nullptr;
             rows[1] = i < w.valid ? p.x_scales + (static_cast<int64_t>(w.t0) + i) * p.ldxs : nullptr;
         };
-        uint4 v[2][2], next[2][2];
-        auto load = [&](uint4 (&to)[2][2]) {
+        uint4 words[2][3], v[2][2];
+        auto load = [&] {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                to[j][0] = to[j][1] = make_uint4(0, 0, 0, 0);
-                if (rows[j]) load_scales(rows[j], kb / 4 * 32, blocks32, p.scale_align, to[j]);
-            }
+            for (int j = 0; j < 2; ++j)
+                load_scale_words(rows[j], kb / 4 * 32, blocks32, j == 0 ? p.w_span : p.x_span, words[j]);
         };
         start_tile();
-        if (t < tiles) load(v);
+        if (t < tiles) load();
         while (t < tiles && ok) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) align_scales(rows[j], kb / 4 * 32, blocks32, words[j], v[j]);
             const int from = kb % 4, to = min(4, w.kb1 - kb / 4 * 4);
             kb = (kb / 4 + 1) * 4;
             if (kb >= w.kb1) {
                 t += tile_step;
                 start_tile();
             }
-            if (t < tiles) load(next);
+            if (t < tiles) load();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 if (q < from || q >= to || !ok) continue;
@@ -423,8 +423,6 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
                 if (lane == 0) ptx::mbar_arrive(&full[ring.stage]);
                 ring.next();
             }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) v[j][0] = next[j][0], v[j][1] = next[j][1];
         }
         __syncwarp();
     }
@@ -515,7 +513,7 @@ int launch_forward_split(const ForwardArgs& f, Operand operand, int splits, uint
     p.zero_rest = f.zero_rest;
     p.x_scales = f.x_scales, p.ldxs = f.ldxs;
     p.w_scales = f.w_scales, p.ws_stride = f.ws_stride, p.ldws = f.ldws;
-    p.scale_align = scale_alignment(f);
+    scale_spans(f, &p.x_span, &p.w_span);
     p.limit_ns = limit_ns, p.status = status;
     static const uint32_t box_rows[3] = {64, 32, 16};
     CUtensorMap a, b[3];

@@ -46,40 +46,68 @@ __device__ __forceinline__ uint32_t scale_word_offset(int r) {
     return static_cast<uint32_t>(r / 128 * 512 + r % 32 * 16 + r % 128 / 32 * 4);
 }
 
-// 32 consecutive scale bytes of a row starting at block `first` of `blocks`
-// (bytes past the end read as zero: any finite scale serves, the codes there
-// are zeros).  The row starts at a multiple of `align` bytes, first is a
-// multiple of 32.
-__device__ __forceinline__ void load_scales(const uint8_t* row, int first, int blocks, int align, uint4 (&out)[2]) {
-    const uint8_t* src = row + first;
-    if (align == 16 && first + 32 <= blocks) {
-        out[0] = __ldg(reinterpret_cast<const uint4*>(src));
-        out[1] = __ldg(reinterpret_cast<const uint4*>(src + 16));
-        return;
-    }
-    uint32_t w[8];
+// The scales of one operand: no byte outside [begin, end) is read.
+struct ScaleSpan {
+    const uint8_t* begin;
+    const uint8_t* end;
+};
+
+// The 16-byte words, aligned, that hold 32 consecutive scale bytes of a row
+// from block `first` (a multiple of 32) of `blocks`: two, or three where the
+// row starts at an odd address.  A word may reach into other rows of the span;
+// what of it lies outside the span reads as zero.  Loads only, so that they can
+// be under way while the thread does something else (byte by byte, rows at odd
+// addresses took 1269 us for 8192 x 8192 x 8224 where 8192 took 276).
+__device__ __forceinline__ void load_scale_words(const uint8_t* row, int first, int blocks, const ScaleSpan& span,
+                                                 uint4 (&out)[3]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int left = blocks - first - 8 * i;
-        uint2 pair = make_uint2(0, 0);
-        if (align >= 8 && left >= 8) {
-            pair = __ldg(reinterpret_cast<const uint2*>(src + 8 * i));
+    for (int c = 0; c < 3; ++c) out[c] = make_uint4(0, 0, 0, 0);
+    if (row == nullptr) return;
+    const int offset = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
+    const int bytes = offset + min(32, blocks - first);
+    const uint8_t* base = row + first - offset;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+        if (16 * c >= bytes) break;
+        const uint8_t* src = base + 16 * c;
+        if (src >= span.begin && src + 16 <= span.end) {
+            out[c] = __ldg(reinterpret_cast<const uint4*>(src));
         } else {
+            uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
-                if (b >= left) break;
-                const uint32_t byte = __ldg(src + 8 * i + b);
-                if (b < 4) {
-                    pair.x |= byte << (8 * b);
-                } else {
-                    pair.y |= byte << (8 * (b - 4));
-                }
-            }
+            for (int b = 0; b < 16; ++b)
+                if (src + b >= span.begin && src + b < span.end)
+                    w[b / 4] |= static_cast<uint32_t>(__ldg(src + b)) << (8 * (b % 4));
+            out[c] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        w[2 * i] = pair.x, w[2 * i + 1] = pair.y;
     }
-    out[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    out[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+// The 32 bytes themselves, from load_scale_words' words; bytes past the row's
+// end are zeros (any finite scale serves, the codes there are zeros).
+__device__ __forceinline__ void align_scales(const uint8_t* row, int first, int blocks, const uint4 (&words)[3],
+                                             uint4 (&out)[2]) {
+    const unsigned offset = static_cast<unsigned>(reinterpret_cast<uintptr_t>(row) & 15);
+    uint32_t q[12] = {words[0].x, words[0].y, words[0].z, words[0].w, words[1].x, words[1].y,
+                      words[1].z, words[1].w, words[2].x, words[2].y, words[2].z, words[2].w};
+    if (offset != 0) {
+#pragma unroll
+        for (int i = 0; i < 10; ++i) q[i] = (offset & 8) ? q[i + 2] : q[i];
+#pragma unroll
+        for (int i = 0; i < 9; ++i) q[i] = (offset & 4) ? q[i + 1] : q[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = __funnelshift_r(q[i], q[i + 1], 8 * (offset & 3));
+    }
+    const int left = blocks - first;
+    if (left < 32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int valid = left - 4 * i;
+            q[i] = valid >= 4 ? q[i] : valid <= 0 ? 0 : q[i] & ((1u << (8 * valid)) - 1);
+        }
+    }
+    out[0] = make_uint4(q[0], q[1], q[2], q[3]);
+    out[1] = make_uint4(q[4], q[5], q[6], q[7]);
 }
 
 // 32 TMEM lanes x 32 columns in the registers of 8 x 8 matrices: after it, r[16
@@ -154,9 +182,8 @@ bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void
 bool encode_forward_maps(const ForwardArgs& f, Operand operand, CUtensorMap* w, CUtensorMap (&x)[3],
                          const uint32_t (&box_rows)[3]);
 
-// Host: the largest of 16, 8 and 1 bytes that every row of scales starts at a
-// multiple of.
-int scale_alignment(const ForwardArgs& f);
+// Host: where the scales of the tokens and of the weights lie.
+void scale_spans(const ForwardArgs& f, ScaleSpan* x, ScaleSpan* w);
 
 }  // namespace grouped
 }  // namespace kmcts

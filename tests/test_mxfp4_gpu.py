@@ -183,10 +183,11 @@ def test_product_random_scales_within_bound(cuda_device, kernel, rows, n, k):
 
 
 @pytest.mark.parametrize("kernel", KERNELS)
-def test_every_block_meets_its_own_scale(cuda_device, kernel):
+@pytest.mark.parametrize("k", [32, 512, 800, 1024, 2048 + 32 * 15, 3200])
+def test_every_block_meets_its_own_scale(cuda_device, kernel, k):
     """One element of 1 in each row, in a block of its own scale: each output
     is one product of two scales, so a scale read from another row or block shows."""
-    rows, n, k = 160, 200, 800
+    rows, n = 160, 200
     a_scales = torch.randint(100, 150, (rows, k // 32), generator=torch.Generator().manual_seed(3), dtype=torch.uint8)
     b_scales = torch.randint(100, 150, (n, k // 32), generator=torch.Generator().manual_seed(4), dtype=torch.uint8)
     a_codes, b_codes = torch.zeros(rows, k // 2, dtype=torch.uint8), torch.full((n, k // 2), 0x22, dtype=torch.uint8)
