@@ -1,8 +1,10 @@
 // CUDA-core kernels of the grouped products, for strides and alignments that
 // TMA cannot take.  One CTA walks 64 x 64 output tiles of the groups; each
-// output is one FP32 accumulator updated by one FMA per step of the contracted
-// dimension in increasing order, rounded once.  Bound by the FP32 units (75
+// output is one FP32 accumulator (FP64 for MXFP4) updated by one FMA per step
+// of the contracted dimension in increasing order, rounded once.  Bound by the FP32 units (75
 // TFLOP/s on B200 at best); the tensor-core kernels take every aligned call.
+#include <type_traits>
+
 #include "grouped_common.cuh"
 
 namespace kmcts {
@@ -13,20 +15,20 @@ constexpr int kTile = 64, kDepth = 16, kThreads = 256;
 
 // acc[i][j] += sum over depth of a(row, d) * b(col, d), for the thread's 4 x 4
 // outputs (rows ty + 16 i, columns tx + 16 j).
-template <typename LoadA, typename LoadB>
-__device__ __forceinline__ void tile_product(float (&acc)[4][4], int rows, int cols, int depth, bool a_depth_inner,
+template <typename T, typename LoadA, typename LoadB>
+__device__ __forceinline__ void tile_product(T (&acc)[4][4], int rows, int cols, int depth, bool a_depth_inner,
                                              bool b_depth_inner, LoadA a, LoadB b) {
-    __shared__ float as[kDepth][kTile + 1];
-    __shared__ float bs[kDepth][kTile + 1];
+    __shared__ T as[kDepth][kTile + 1];
+    __shared__ T bs[kDepth][kTile + 1];
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
     for (int d0 = 0; d0 < depth; d0 += kDepth) {
         for (int i = threadIdx.x; i < kDepth * kTile; i += kThreads) {
             int d = a_depth_inner ? i % kDepth : i / kTile;
             int r = a_depth_inner ? i / kDepth : i % kTile;
-            as[d][r] = r < rows && d0 + d < depth ? a(r, d0 + d) : 0.0f;
+            as[d][r] = r < rows && d0 + d < depth ? a(r, d0 + d) : T(0);
             d = b_depth_inner ? i % kDepth : i / kTile;
             r = b_depth_inner ? i / kDepth : i % kTile;
-            bs[d][r] = r < cols && d0 + d < depth ? b(r, d0 + d) : 0.0f;
+            bs[d][r] = r < cols && d0 + d < depth ? b(r, d0 + d) : T(0);
         }
         __syncthreads();
         const int steps = min(kDepth, depth - d0);  // no step past the end: 0 * inf must not enter
@@ -35,10 +37,13 @@ __device__ __forceinline__ void tile_product(float (&acc)[4][4], int rows, int c
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __fmaf_rn(as[d][ty + 16 * i], bs[d][tx + 16 * j], acc[i][j]);
+                    acc[i][j] = fma(as[d][ty + 16 * i], bs[d][tx + 16 * j], acc[i][j]);
         __syncthreads();
     }
 }
+
+__device__ __forceinline__ __nv_bfloat16 rounded(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ __nv_bfloat16 rounded(double v) { return __double2bfloat16(v); }
 
 template <Operand KIND>
 __global__ void __launch_bounds__(kThreads) grouped_forward_simt(ForwardArgs p) {
@@ -57,14 +62,16 @@ __global__ void __launch_bounds__(kThreads) grouped_forward_simt(ForwardArgs p) 
         const int col0 = in_group % tiles_n * kTile;
         const int rows = min(kTile, static_cast<int>(table.row[e + 1] - row0));
         const int cols = min(kTile, p.n - col0);
-        float acc[4][4] = {};
+        // MXFP4 values reach 6 * 2^127 and products 2^256: FP64 holds them.
+        using Sum = std::conditional_t<KIND == Operand::kMxfp4, double, float>;
+        Sum acc[4][4] = {};
         if constexpr (KIND == Operand::kMxfp4) {
             auto* x = static_cast<const uint8_t*>(p.x) + row0 * p.ldx;
             auto* xs = p.x_scales + row0 * p.ldxs;
             auto* w = static_cast<const uint8_t*>(p.w) + e * p.w_stride + col0 * p.ldw;
             auto* ws = p.w_scales + e * p.ws_stride + col0 * p.ldws;
             auto value = [](const uint8_t* codes, const uint8_t* scales, int d) {
-                return e2m1_value(codes[d / 2] >> (d % 2 * 4)) * e8m0_value(scales[d / 32]);
+                return static_cast<double>(e2m1_value(codes[d / 2] >> (d % 2 * 4))) * e8m0_value(scales[d / 32]);
             };
             tile_product(
                 acc, rows, cols, p.k, true, true, [&](int r, int d) { return value(x + r * p.ldx, xs + r * p.ldxs, d); },
@@ -84,7 +91,7 @@ __global__ void __launch_bounds__(kThreads) grouped_forward_simt(ForwardArgs p) 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int r = threadIdx.x / 16 + 16 * i, c = threadIdx.x % 16 + 16 * j;
-                if (r < rows && c < cols) y[(row0 + r) * p.ldy + col0 + c] = __float2bfloat16_rn(acc[i][j]);
+                if (r < rows && c < cols) y[(row0 + r) * p.ldy + col0 + c] = rounded(acc[i][j]);
             }
     }
     if (p.zero_rest) zero_rest_rows(y, p.ldy, table.rows(), p.rows, p.n, blockIdx.x, gridDim.x);

@@ -152,9 +152,10 @@ def _strided_rows(t: torch.Tensor) -> torch.Tensor:
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, ends):
+    def forward(ctx, x, w, ends, code):
         ctx.save_for_backward(x, w, ends)
-        return grouped_gemm(x, w, ends)
+        ctx.code = code
+        return grouped_gemm(x, w, ends, w_layout=code)
 
     @staticmethod
     def backward(ctx, dy):
@@ -162,17 +163,20 @@ class _GroupedLinear(torch.autograd.Function):
             raise RuntimeError("grouped_linear is differentiable once")
         x, w, ends = ctx.saved_tensors
         dy = _strided_rows(dy)
-        dx = grouped_gemm(dy, w, ends, w_layout="row") if ctx.needs_input_grad[0] else None
-        dw = grouped_gemm_wgrad(dy, x, ends) if ctx.needs_input_grad[1] else None
-        return dx, dw, None
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = grouped_gemm(dy, w, ends, w_layout=1 - ctx.code)
+        if ctx.needs_input_grad[1]:
+            dw = grouped_gemm_wgrad(dy, x, ends) if ctx.code == _native.B_COL else grouped_gemm_wgrad(x, dy, ends)
+        return dx, dw, None, None
 
 
-def grouped_linear(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
-    """Differentiable ``grouped_gemm(x, w, ends)`` for ``w`` of ``[groups, N, K]``.
+def grouped_linear(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *, w_layout: str | int = "col") -> torch.Tensor:
+    """Differentiable ``grouped_gemm(x, w, ends, w_layout=w_layout)``.
 
     The gradients of ``x`` and ``w`` are bfloat16; ``x``'s is zero in rows
     behind the last group.  Once differentiable."""
-    return _GroupedLinear.apply(x, w, ends)
+    return _GroupedLinear.apply(x, w, ends, layout_code(w_layout))
 
 
 __all__ = ["grouped_gemm", "grouped_gemm_wgrad", "grouped_linear"]

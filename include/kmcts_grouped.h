@@ -80,7 +80,8 @@ int kmcts_mxfp4_quantize(const void* X, int x_type, int64_t ldx, void* codes, in
                          int64_t rows, int K, void* stream);
 
 /* out[r, k] = value of the code times its block's scale, rounded once to
- * out_type (exact in FP32 and, above 2^-133, in BF16). */
+ * out_type (exact in FP32 and, from 2^-133 up, in BF16; an infinity where the
+ * type ends: 2^128, in FP16 2^16). */
 int kmcts_mxfp4_dequantize(const void* codes, int64_t ldc, const void* scales, int64_t lds, void* out, int out_type,
                            int64_t ldo, int64_t rows, int K, void* stream);
 

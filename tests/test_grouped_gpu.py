@@ -258,6 +258,97 @@ def test_linear_gradients(cuda_device):
         assert (loss(x.detach(), moved) - base).to(torch.bfloat16) == gw[e, i, j]
 
 
+def test_linear_gradients_of_a_row_major_weight(cuda_device):
+    counts, n, k = [33, 0, 140, 7], 72, 104
+    x, w = integers(190, k, seed=1).requires_grad_(), integers(4, k, n, seed=2).requires_grad_()
+    y = grouped.grouped_linear(x, w, ends_of(counts), w_layout="row")
+    dy = integers(190, n, seed=3)
+    gx, gw = torch.autograd.grad(y, (x, w), dy)
+    assert torch.equal(y, forward64(x.detach(), w.detach(), counts, "row")[0].to(torch.bfloat16))
+    assert torch.equal(gx, forward64(dy, w.detach(), counts, "col")[0].to(torch.bfloat16))
+    assert torch.equal(gw, wgrad64(x.detach(), dy, counts)[0].to(torch.bfloat16))
+
+
+def test_step_as_a_graph(cuda_device):
+    """Forward and backward captured together, after the usual warm-up on a
+    side stream, and replayed on other data and other groups."""
+    n, k = 136, 256
+    x, w = integers(300, k, seed=1).requires_grad_(), integers(3, n, k, seed=2).requires_grad_()
+    dy, ends = integers(300, n, seed=3), ends_of([100, 150, 50])
+
+    def step():
+        y = grouped.grouped_linear(x, w, ends)
+        return (y, *torch.autograd.grad(y, (x, w), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, gx, gw = step()
+    counts = [17, 0, 260]
+    with torch.no_grad():
+        x.copy_(integers(300, k, seed=4))
+        ends.copy_(ends_of(counts))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, forward64(x.detach(), w.detach(), counts, "col")[0].to(torch.bfloat16))
+    assert torch.equal(gx, forward64(dy, w.detach(), counts, "row")[0].to(torch.bfloat16))
+    assert torch.equal(gw, wgrad64(dy, x.detach(), counts)[0].to(torch.bfloat16))
+
+
+def test_two_streams_at_once(cuda_device):
+    """Calls that overlap on the GPU share nothing."""
+    counts, n, k = [700, 30, 300], 512, 1024
+    x, w, ends = integers(1030, k, seed=1), integers(3, n, k, seed=2), ends_of(counts)
+    few, few_ends = integers(9, k, seed=3), ends_of([4, 0, 5])
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    results = [[], [], []]
+    for _ in range(6):
+        results[0].append(grouped.grouped_gemm(x, w, ends, stream=streams[0]))
+        results[1].append(grouped.grouped_gemm(few, w, few_ends, kernel="split", stream=streams[1]))
+        results[2].append(grouped.grouped_gemm_wgrad(x[:, :n], x, ends, stream=streams[2]))
+    torch.cuda.synchronize()
+    refs = (forward64(x, w, counts, "col")[0].to(torch.bfloat16),
+            forward64(few, w, [4, 0, 5], "col")[0].to(torch.bfloat16),
+            wgrad64(x[:, :n], x, counts)[0].to(torch.bfloat16))
+    for got, ref in zip(results, refs):
+        assert all(torch.equal(g, ref) for g in got)
+
+
+def test_one_weight_for_all_groups(cuda_device):
+    """A weight expanded over the groups (stride 0)."""
+    counts, n, k = [40, 3, 90], 128, 256
+    x, w = integers(133, k, seed=1), integers(1, n, k, seed=2).expand(3, n, k)
+    y = checked(grouped.grouped_gemm, x, w, ends_of(counts))
+    assert torch.equal(y, forward64(x, w, counts, "col")[0].to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_offsets_past_32_bits(cuda_device, kernel):
+    """Rows of x and y, and groups of w, more than 2^31 elements apart."""
+    rows, n, k, far = 70, 72, 64, 2 ** 25 + 8
+    x_store = torch.zeros(rows * far, dtype=torch.bfloat16, device="cuda")
+    y_store = torch.zeros(rows * far, dtype=torch.bfloat16, device="cuda")
+    x, y = (t.as_strided((rows, c), (far, 1)) for t, c in ((x_store, k), (y_store, n)))
+    x.copy_(integers(rows, k, seed=1))
+    w = y_store.as_strided((3, n, k), (2 ** 30 + 2 ** 20, k, 1), 128)  # groups 2^30 apart, clear of y's rows
+    w.copy_(integers(3, n, k, seed=2))
+    counts = [30, 0, 40]
+    ref = forward64(x, w, counts, "col")[0].to(torch.bfloat16)
+    checked(grouped.grouped_gemm, x, w.clone() if kernel == "simt" else w, ends_of(counts), y, kernel=kernel)
+    assert torch.equal(y, ref)
+    gradient = x_store.as_strided((3, n, k), (2 ** 30 + 2 ** 20, k, 1), 128)
+    dy = integers(rows, n, seed=3)
+    dw_kernel = kernel if kernel in GRADIENT_KERNELS else "auto"
+    checked(grouped.grouped_gemm_wgrad, dy, x, ends_of(counts), gradient, kernel=dw_kernel)
+    assert torch.equal(gradient, wgrad64(dy, x, counts)[0].to(torch.bfloat16))
+
+
 def test_only_the_gradients_asked_for_are_computed(cuda_device):
     x, w = integers(8, 16, seed=1), integers(1, 8, 16, seed=2).requires_grad_()
     y = grouped.grouped_linear(x, w, ends_of([8]))

@@ -199,6 +199,23 @@ def test_every_block_meets_its_own_scale(cuda_device, kernel, k):
 
 
 @pytest.mark.parametrize("kernel", KERNELS)
+def test_extreme_scales(cuda_device, kernel):
+    """Scales at the ends of their range whose products are in the middle, and
+    products past the range of the result."""
+    rows, n, k = 40, 72, 64
+    a, b = random_pair(rows, k, seed=1), random_pair(n, k, seed=2)
+    for sa, sb in ((0, 254), (254, 0), (1, 253), (20, 230)):
+        a.scales.fill_(sa)
+        b.scales.fill_(sb)
+        assert torch.equal(checked(a, b, kernel=kernel), product64(a, b)[0].to(torch.bfloat16)), (sa, sb)
+    a.scales.fill_(254)
+    b.scales.fill_(200)
+    ref = product64(a, b)[0].to(torch.bfloat16)
+    y = checked(a, b, kernel=kernel)
+    assert torch.equal(y.isinf(), ref.isinf()) and torch.equal(y, ref)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("counts", [[1], [0, 1, 127, 0, 128, 129, 15, 16, 17, 0], [600, 0, 257, 3], [0, 0]])
 @pytest.mark.parametrize("n,k", [(128, 256), (77, 96), (264, 800)])
 def test_grouped_product_bit_exact(cuda_device, kernel, counts, n, k):
