@@ -11,23 +11,30 @@ namespace kmcts {
 namespace grouped {
 
 // First row and first tile of every group, and one past the last, in shared
-// memory: 2 x (groups + 1) ints.
+// memory (2 x (groups + 1) ints), and where the kernel splits a group's rows
+// evenly over its tiles, the rows of one (another groups + 1).
 struct GroupTable {
     int* row;
     int* tile;
+    int* step;
     int groups;
 
+    __device__ GroupTable(int* smem, int count)
+        : row(smem), tile(smem + count + 1), step(smem + 2 * (count + 1)), groups(count) {}
     __device__ int tiles() const { return tile[groups]; }
     __device__ int rows() const { return row[groups]; }
 };
 
+constexpr int table_bytes(int groups, bool steps) { return (steps ? 3 : 2) * 4 * (groups + 1); }
+
 // Built by one whole warp: a running maximum of the ends, clamped to the
 // rows there are, and a running sum of tiles_of(rows of the group).  Ends out
 // of order or out of range thus only make groups empty or short.  ends ==
-// nullptr is one group of all rows.
+// nullptr is one group of all rows.  unit > 0: also the rows of a tile, a
+// multiple of unit, for groups of max_step rows a tile at most.
 template <typename TilesOf>
 __device__ __forceinline__ void build_group_table(const GroupTable& t, const int32_t* ends, int rows,
-                                                  TilesOf tiles_of) {
+                                                  TilesOf tiles_of, int max_step = 0, int unit = 0) {
     const int lane = threadIdx.x & 31;
     int last_end = 0, last_tile = 0;
     for (int base = 0; base < t.groups; base += 32) {
@@ -51,6 +58,10 @@ __device__ __forceinline__ void build_group_table(const GroupTable& t, const int
         }
         if (e < t.groups) {
             t.row[e] = start;
+            if (unit > 0 && end > start) {
+                const int each = (end - start - 1) / ((end - start + max_step - 1) / max_step) + 1;
+                t.step[e] = (each + unit - 1) / unit * unit;
+            }
             t.tile[e] = last_tile + sum - mine;
         }
         last_end = __shfl_sync(0xffffffffu, end, 31);

@@ -59,7 +59,7 @@ struct Pair {
     static constexpr int kStagingOffset = kStages * kStageBytes;
     static constexpr int kBarrierOffset = kStagingOffset + kEpilogueWarps * kStagingBytes;
     static constexpr int kTableOffset = kBarrierOffset + 512;
-    static constexpr int smem_bytes(int groups) { return 1024 + kTableOffset + 8 * (groups + 1); }
+    static constexpr int smem_bytes(int groups) { return 1024 + kTableOffset + table_bytes(groups, !kGrad); }
     static_assert(2 * kMaxWidth + (kMx ? kStages * kScaleCols : 0) <= 512, "TMEM columns");
     static_assert(smem_bytes(KMCTS_MAX_GROUPS) <= kMaxSmem, "shared memory");
 };
@@ -79,6 +79,7 @@ struct PairParams {
     const uint8_t* w_scales;
     int64_t ws_stride, ldws;
     ScaleSpan x_span, w_span;
+    Divisor strip;  // eight rows of tiles
     uint64_t limit_ns;
     int* status;
 };
@@ -98,8 +99,7 @@ __device__ __forceinline__ Tile tile_at(const GroupTable& table, const PairParam
     const int in_group = t - table.tile[out.e];
     const int first = table.row[out.e], rows = table.row[out.e + 1] - first;
     if constexpr (L::kGrad) {
-        const int tiles_k = (p.k + L::kMaxWidth - 1) / L::kMaxWidth;
-        const TileCoord tc = tile_coord(in_group, (p.n + 255) / 256, tiles_k, 8);
+        const TileCoord tc = raster(in_group, (p.n + 255) / 256, p.strip);
         out.n0 = tc.m_blk * 256;
         out.b0 = tc.n_blk * L::kMaxWidth;
         out.valid = min(L::kMaxWidth, p.k - out.b0);
@@ -108,8 +108,8 @@ __device__ __forceinline__ Tile tile_at(const GroupTable& table, const PairParam
         out.tail = rows % L::kBK;
     } else {
         const int tiles_t = (rows + L::kMaxWidth - 1) / L::kMaxWidth;
-        const int step = round_up((rows + tiles_t - 1) / tiles_t, 32);
-        const TileCoord tc = tile_coord(in_group, tiles_t, (p.n + 255) / 256, 8);
+        const int step = table.step[out.e];
+        const TileCoord tc = raster(in_group, tiles_t, p.strip);
         out.n0 = tc.n_blk * 256;
         out.b0 = first + tc.m_blk * step;
         out.valid = min(step, first + rows - out.b0);
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* no_abort = abort + 1;
     int* table_smem = reinterpret_cast<int*>(smem + L::kTableOffset);
-    const GroupTable table = {table_smem, table_smem + p.groups + 1, p.groups};
+    const GroupTable table(table_smem, p.groups);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = static_cast<int>(ptx::cluster_ctarank());
@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
             build_group_table(table, p.ends, p.rows, [&](int) { return per_group; });
         } else {
             build_group_table(table, p.ends, p.rows,
-                              [&](int rows) { return (rows + L::kMaxWidth - 1) / L::kMaxWidth * tiles_a; });
+                              [&](int rows) { return (rows + L::kMaxWidth - 1) / L::kMaxWidth * tiles_a; }, L::kMaxWidth,
+                              32);
         }
     }
     __syncwarp();
@@ -679,6 +680,7 @@ int launch_forward_pair(const ForwardArgs& f, Operand operand, uint64_t limit_ns
     const uint32_t box_rows[3] = {mx ? 96u : 128u, 64, 32};
     CUtensorMap a, b[3];
     if (!encode_forward_maps(f, operand, &a, b, box_rows)) return KMCTS_ENOTSUP;
+    p.strip = Divisor::of(8 * ((f.n + 255) / 256));
     const int64_t width = mx ? 192 : 256;
     const int64_t tiles = (f.rows / width + f.groups) * ((f.n + 255) / 256);
     if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;
@@ -713,6 +715,7 @@ int launch_wgrad_pair(const WgradArgs& g, uint64_t limit_ns, cudaStream_t stream
                         strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
             return KMCTS_ENOTSUP;
     }
+    p.strip = Divisor::of(8 * ((g.k + 255) / 256));
     p.stream_out = static_cast<int64_t>(g.groups) * g.n * g.k * (g.fp32 ? 4 : 2) > 63LL << 20;  // L2 is 126 MB
     const int64_t tiles = static_cast<int64_t>(g.groups) * ((g.n + 255) / 256) * ((g.k + 255) / 256);
     if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;

@@ -48,7 +48,7 @@ __device__ __forceinline__ __nv_bfloat16 rounded(double v) { return __double2bfl
 template <Operand KIND>
 __global__ void __launch_bounds__(kThreads) grouped_forward_simt(ForwardArgs p) {
     extern __shared__ int table_smem[];
-    const GroupTable table = {table_smem, table_smem + p.groups + 1, p.groups};
+    const GroupTable table(table_smem, p.groups);
     const int tiles_n = (p.n + kTile - 1) / kTile;
     if (threadIdx.x < 32)
         build_group_table(table, p.ends, p.rows, [&](int rows) { return (rows + kTile - 1) / kTile * tiles_n; });
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kThreads) grouped_forward_simt(ForwardArgs p) 
 
 __global__ void __launch_bounds__(kThreads) grouped_wgrad_simt(WgradArgs p) {
     extern __shared__ int table_smem[];
-    const GroupTable table = {table_smem, table_smem + p.groups + 1, p.groups};
+    const GroupTable table(table_smem, p.groups);
     const int tiles_k = (p.k + kTile - 1) / kTile;
     const int per_group = (p.n + kTile - 1) / kTile * tiles_k;
     if (threadIdx.x < 32) build_group_table(table, p.ends, p.rows, [&](int) { return per_group; });
@@ -133,8 +133,6 @@ __global__ void __launch_bounds__(kThreads) grouped_wgrad_simt(WgradArgs p) {
     }
 }
 
-size_t table_bytes(int groups) { return 2 * sizeof(int) * (groups + 1); }
-
 unsigned grid_for(int64_t tiles) {
     const int64_t most = 8LL * multiprocessor_count();
     return static_cast<unsigned>(tiles < 1 ? 1 : tiles < most ? tiles : most);
@@ -149,13 +147,13 @@ int launch_forward_simt(const ForwardArgs& a, Operand kind, cudaStream_t stream)
     const unsigned grid = grid_for(tiles);
     switch (kind) {
         case Operand::kBf16Col:
-            grouped_forward_simt<Operand::kBf16Col><<<grid, kThreads, table_bytes(a.groups), stream>>>(a);
+            grouped_forward_simt<Operand::kBf16Col><<<grid, kThreads, table_bytes(a.groups, false), stream>>>(a);
             break;
         case Operand::kBf16Row:
-            grouped_forward_simt<Operand::kBf16Row><<<grid, kThreads, table_bytes(a.groups), stream>>>(a);
+            grouped_forward_simt<Operand::kBf16Row><<<grid, kThreads, table_bytes(a.groups, false), stream>>>(a);
             break;
         case Operand::kMxfp4:
-            grouped_forward_simt<Operand::kMxfp4><<<grid, kThreads, table_bytes(a.groups), stream>>>(a);
+            grouped_forward_simt<Operand::kMxfp4><<<grid, kThreads, table_bytes(a.groups, false), stream>>>(a);
             break;
     }
     g_launches.fetch_add(1, std::memory_order_relaxed);
@@ -165,7 +163,7 @@ int launch_forward_simt(const ForwardArgs& a, Operand kind, cudaStream_t stream)
 int launch_wgrad_simt(const WgradArgs& a, cudaStream_t stream) {
     const int64_t tiles = static_cast<int64_t>(a.groups) * ((a.n + kTile - 1) / kTile) * ((a.k + kTile - 1) / kTile);
     if (tiles > 0x7fffffff) return KMCTS_ENOTSUP;
-    grouped_wgrad_simt<<<grid_for(tiles), kThreads, table_bytes(a.groups), stream>>>(a);
+    grouped_wgrad_simt<<<grid_for(tiles), kThreads, table_bytes(a.groups, false), stream>>>(a);
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return cudaGetLastError() == cudaSuccess ? KMCTS_OK : KMCTS_EGEMM;
 }

@@ -43,7 +43,7 @@ struct Split {
     static constexpr int kPartsOffset = kStages * kStageBytes;
     static constexpr int kBarrierOffset = kPartsOffset + 4 * kPartBytes;
     static constexpr int kTableOffset = kBarrierOffset + 512;
-    static constexpr int smem_bytes(int groups) { return 1024 + kTableOffset + 8 * (groups + 1); }
+    static constexpr int smem_bytes(int groups) { return 1024 + kTableOffset + table_bytes(groups, false); }
     static_assert(2 * kMaxWidth + (kMx ? kStages * kScaleCols : 0) <= kTmemCols, "TMEM columns");
     static_assert(smem_bytes(KMCTS_MAX_GROUPS) <= kMaxSmem, "shared memory");
 };
@@ -77,15 +77,18 @@ __device__ __forceinline__ Tile tile_at(const GroupTable& table, const SplitPara
     const int in_group = t - table.tile[out.e];
     const int first = table.row[out.e], rows = table.row[out.e + 1] - first;
     const int tiles_t = (rows + kMaxWidth - 1) / kMaxWidth;
-    const int step = round_up((rows + tiles_t - 1) / tiles_t, 16);
-    // A weight tile's token tiles follow one another: its second reading is from L2.
-    out.n0 = in_group / tiles_t * 128;
-    out.t0 = first + in_group % tiles_t * step;
+    const int step = tiles_t == 1 ? round_up(rows, 16) : round_up((rows + tiles_t - 1) / tiles_t, 16);
+    // A weight tile's token tiles follow one another: its second reading is
+    // from L2.
+    const int n_blk = tiles_t == 1 ? in_group : in_group / tiles_t;
+    out.n0 = n_blk * 128;
+    out.t0 = first + (in_group - n_blk * tiles_t) * step;
     out.valid = min(step, first + rows - out.t0);
     out.width = round_up(out.valid, 16);
-    const int blocks = (p.k + Split<KIND>::kBK - 1) / Split<KIND>::kBK;
-    out.kb0 = rank * blocks / splits;
-    out.kb1 = (rank + 1) * blocks / splits;
+    // Splits are 1, 2 or 4.
+    const int blocks = (p.k + Split<KIND>::kBK - 1) / Split<KIND>::kBK, shift = splits >> 1;
+    out.kb0 = static_cast<int>(static_cast<int64_t>(rank) * blocks >> shift);
+    out.kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * blocks >> shift);
     return out;
 }
 
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* no_abort = abort + 1;
     int* table_smem = reinterpret_cast<int*>(smem + L::kTableOffset);
-    const GroupTable table = {table_smem, table_smem + p.groups + 1, p.groups};
+    const GroupTable table(table_smem, p.groups);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = static_cast<int>(ptx::cluster_ctarank());
