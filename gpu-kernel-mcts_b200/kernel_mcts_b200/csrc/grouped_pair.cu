@@ -79,7 +79,8 @@ struct PairParams {
     const uint8_t* w_scales;
     int64_t ws_stride, ldws;
     ScaleSpan x_span, w_span;
-    Divisor strip;  // eight rows of tiles
+    Divisor strip;      // eight rows of tiles
+    Divisor per_group;  // gradient: tiles of a group
     uint64_t limit_ns;
     int* status;
 };
@@ -95,11 +96,14 @@ template <Kind KIND>
 __device__ __forceinline__ Tile tile_at(const GroupTable& table, const PairParams& p, int t, int& group) {
     using L = Pair<KIND>;
     Tile out = {};
-    out.e = group_of_tile(table, t, group);
-    const int in_group = t - table.tile[out.e];
+    if constexpr (L::kGrad) {
+        out.e = static_cast<int>(p.per_group.quotient(t));
+    } else {
+        out.e = group_of_tile(table, t, group);
+    }
     const int first = table.row[out.e], rows = table.row[out.e + 1] - first;
     if constexpr (L::kGrad) {
-        const TileCoord tc = raster(in_group, (p.n + 255) / 256, p.strip);
+        const TileCoord tc = raster(t - out.e * p.per_group.d, (p.n + 255) / 256, p.strip);
         out.n0 = tc.m_blk * 256;
         out.b0 = tc.n_blk * L::kMaxWidth;
         out.valid = min(L::kMaxWidth, p.k - out.b0);
@@ -109,7 +113,7 @@ __device__ __forceinline__ Tile tile_at(const GroupTable& table, const PairParam
     } else {
         const int tiles_t = (rows + L::kMaxWidth - 1) / L::kMaxWidth;
         const int step = table.step[out.e];
-        const TileCoord tc = raster(in_group, tiles_t, p.strip);
+        const TileCoord tc = raster(t - table.tile[out.e], tiles_t, p.strip);
         out.n0 = tc.n_blk * 256;
         out.b0 = first + tc.m_blk * step;
         out.valid = min(step, first + rows - out.b0);
@@ -693,6 +697,8 @@ int launch_forward_pair(const ForwardArgs& f, Operand operand, uint64_t limit_ns
 }
 
 int launch_wgrad_pair(const WgradArgs& g, uint64_t limit_ns, cudaStream_t stream, int* status) {
+    const int64_t tiles = static_cast<int64_t>(g.groups) * ((g.n + 255) / 256) * ((g.k + 255) / 256);
+    if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;
     PairParams p = {};
     p.ends = g.ends, p.groups = g.groups, p.rows = g.rows, p.n = g.n, p.k = g.k;
     p.fp32 = g.fp32, p.accumulate = g.accumulate;
@@ -716,9 +722,8 @@ int launch_wgrad_pair(const WgradArgs& g, uint64_t limit_ns, cudaStream_t stream
             return KMCTS_ENOTSUP;
     }
     p.strip = Divisor::of(8 * ((g.k + 255) / 256));
+    p.per_group = Divisor::of(static_cast<uint32_t>(tiles / g.groups));
     p.stream_out = static_cast<int64_t>(g.groups) * g.n * g.k * (g.fp32 ? 4 : 2) > 63LL << 20;  // L2 is 126 MB
-    const int64_t tiles = static_cast<int64_t>(g.groups) * ((g.n + 255) / 256) * ((g.k + 255) / 256);
-    if (tiles >= 1LL << 30) return KMCTS_ENOTSUP;
     return launch<Kind::kWgrad>(a, b, c, p, tiles, stream);
 }
 
