@@ -73,6 +73,28 @@ __device__ __forceinline__ void build_group_table(const GroupTable& t, const int
     }
 }
 
+// The first rows alone, of `count` groups from `first` on (row[count] is one
+// past the last): for kernels whose groups all have the same number of tiles.
+__device__ __forceinline__ void build_group_rows(int* row, const int32_t* ends, int rows, int first, int count) {
+    const int lane = threadIdx.x & 31;
+    int last_end = 0;
+    for (int base = 0; base < first + count; base += 32) {
+        const int e = base + lane;
+        int end = e < first + count ? min(max(ends[e], 0), rows) : 0;
+        if (lane == 0) end = max(end, last_end);
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int other = __shfl_up_sync(0xffffffffu, end, d);
+            if (lane >= d) end = max(end, other);
+        }
+        int start = __shfl_up_sync(0xffffffffu, end, 1);
+        if (lane == 0) start = last_end;
+        if (e >= first && e < first + count) row[e - first] = start;
+        last_end = __shfl_sync(0xffffffffu, end, 31);
+    }
+    if (lane == 0) row[count] = last_end;
+}
+
 // The group that tile `t` belongs to (the one group with tile[e] <= t <
 // tile[e + 1]).  A CTA's tiles come in increasing order, so the search goes on
 // from the last tile's group; a search from the start cost a tile more than

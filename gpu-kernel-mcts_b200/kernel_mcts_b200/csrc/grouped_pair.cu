@@ -10,7 +10,7 @@
 //
 // The weights' gradient (Kind::kWgrad) is the same pipeline with the output
 // gradient's columns as A, the input's as B, both MN-major, and the group's
-// rows as the contracted dimension.  Its last block of 64 rows may reach into
+// rows as the contracted dimension.  Its last stage of 128 rows may reach into
 // the next group: a warp of each CTA zeroes the foreign rows of the last
 // 16-row step in shared memory (both operands: 0 * inf is not 0), and the MMA
 // takes no further step.
@@ -39,10 +39,12 @@ struct Pair {
     static constexpr bool kGrad = KIND == Kind::kWgrad;
     static constexpr bool kAMn = KIND == Kind::kRow || kGrad;  // A (and for the gradient B) MN-major
     static constexpr int kThreads = kBaseThreads + (kMx ? 160 : kGrad ? 32 : 0);
-    // K elements of a stage: 128 bytes a row, or two such blocks.  (BF16
-    // forward products with six stages of one block took 3 to 8% longer than
-    // with three of two: 16 experts, 8192 rows, 4096 x 4096, 236 us against 228.)
-    static constexpr int kBlocks = kMx || kGrad ? 1 : 2;
+    // K elements of a stage: a block (256 in MXFP4, 64 in BF16: 128 bytes of
+    // a K-major row), or two.  BF16 forward products with six stages of one
+    // block took 3 to 8% longer than with three of two (16 experts, 8192 rows,
+    // 4096 x 4096: 236 us against 228), gradients with five of one 7 to 17%
+    // (16 groups of 512 rows: 252 us against 234, one of 8192: 234 against 200).
+    static constexpr int kBlocks = kMx ? 1 : 2;
     static constexpr int kBK = kMx ? 256 : 64 * kBlocks;
     static constexpr int kMaxWidth = kMx ? 192 : 256;
     static constexpr int kABlock = 128 * 128;  // bytes of one block, B's for the widest tile
@@ -53,20 +55,25 @@ struct Pair {
     static constexpr int kScaleBytes = kMx ? 2 * 512 + 2 * 1024 : 0;
     static constexpr int kStageBytes = kABytes + kBBytes + kScaleBytes;
     // MXFP4: each stage's scales have TMEM columns of their own, 8 + 16.
-    static constexpr int kStages = kMx || kGrad ? 5 : 3;
+    static constexpr int kStages = kMx ? 5 : 3;
     static constexpr int kScaleCols = 24;
     static constexpr int kStagingBytes = kGrad ? 4096 : 2048;  // an epilogue warp's
     static constexpr int kStagingOffset = kStages * kStageBytes;
     static constexpr int kBarrierOffset = kStagingOffset + kEpilogueWarps * kStagingBytes;
     static constexpr int kTableOffset = kBarrierOffset + 512;
-    static constexpr int smem_bytes(int groups) { return 1024 + kTableOffset + table_bytes(groups, !kGrad); }
+    // The gradient's table holds first rows only, and of so many groups a launch.
+    static constexpr int kMaxGroups = kGrad ? 256 : KMCTS_MAX_GROUPS;
+    static constexpr int smem_bytes(int groups) {
+        return 1024 + kTableOffset + (kGrad ? 4 * (groups + 1) : table_bytes(groups, true));
+    }
     static_assert(2 * kMaxWidth + (kMx ? kStages * kScaleCols : 0) <= 512, "TMEM columns");
-    static_assert(smem_bytes(KMCTS_MAX_GROUPS) <= kMaxSmem, "shared memory");
+    static_assert(smem_bytes(kMaxGroups) <= kMaxSmem, "shared memory");
 };
 
 struct PairParams {
     const int32_t* ends;
     int groups, rows;
+    int first_group;    // gradient: of this launch
     int n, k;           // the weight is n x k (MMA: n in A's rows; gradient: k in B's columns)
     __nv_bfloat16* y;   // forward output
     int64_t ldy;
@@ -89,7 +96,7 @@ struct PairParams {
 // from b0, `width` of them computed and `valid` stored, over `blocks` stages.
 struct Tile {
     int e, n0, b0, width, valid, blocks;
-    int t0, tail;  // gradient: first contracted row, rows of the last block (0: full)
+    int t0, tail;  // gradient: first contracted row, rows of the last stage (0: full)
 };
 
 template <Kind KIND>
@@ -127,7 +134,7 @@ struct Barriers {
     uint64_t *full, *empty;            // a stage's operands are here; its MMAs are done
     uint64_t *tmem_full, *tmem_empty;  // an accumulator is complete; it has been read
     uint64_t* drain;                   // every MMA is done
-    uint64_t *landed, *fixed;          // gradient: a ragged block is here; its tail is zeroed
+    uint64_t *landed, *fixed;          // gradient: a ragged stage is here; its tail is zeroed
     uint64_t *copied, *copies_done;    // MXFP4: a stage's scales are in TMEM; all of them are
 };
 
@@ -197,11 +204,10 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
     // Up to here the launch overlaps the end of the grid before.
     ptx::wait_for_earlier_grids();
     if (warp == 2) {
-        const int tiles_a = (p.n + 255) / 256;
         if constexpr (L::kGrad) {
-            const int per_group = tiles_a * ((p.k + L::kMaxWidth - 1) / L::kMaxWidth);
-            build_group_table(table, p.ends, p.rows, [&](int) { return per_group; });
+            build_group_rows(table.row, p.ends, p.rows, p.first_group, p.groups);
         } else {
+            const int tiles_a = (p.n + 255) / 256;
             build_group_table(table, p.ends, p.rows,
                               [&](int rows) { return (rows + L::kMaxWidth - 1) / L::kMaxWidth * tiles_a; }, L::kMaxWidth,
                               32);
@@ -213,7 +219,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
     ptx::cluster_sync();  // the leader's barriers exist before the peer signals them
     ptx::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int tiles = table.tiles();
+    const int tiles = L::kGrad ? p.groups * static_cast<int>(p.per_group.d) : table.tiles();
     int group = 0;  // the last tile's
     constexpr int kAccStep = L::kMx ? 192 : kAccCols;
 
@@ -233,7 +239,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                 const int boxes = (half + 63) / 64;
                 const CUtensorMap* mb = half > 64 ? &map_b128 : half > 32 ? &map_b64 : &map_b32;
                 const int box_rows = half > 64 ? L::kMaxWidth / 2 : half > 32 ? 64 : 32;
-                const uint32_t b_bytes = static_cast<uint32_t>(L::kGrad ? boxes * 8192 : box_rows * 128 * L::kBlocks);
+                const uint32_t b_bytes = static_cast<uint32_t>(L::kGrad ? boxes * 8192 : box_rows * 128);  // of a block
                 for (int kb = 0; kb < w.blocks; ++kb) {
                     if (!ptx::mbar_wait(&bar.empty[ring.stage], ring.phase ^ 1u, p.limit_ns, abort)) {
                         record_failure(p.status, abort, kRoleProducer);
@@ -244,21 +250,26 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                     uint8_t* sb = sa + L::kABytes;
                     uint32_t full = ptx::mapa_shared(ptx::smem_addr(&bar.full[ring.stage]), 0);
                     if constexpr (L::kGrad) {
-                        // A ragged last block lands on this CTA's own barrier:
+                        // A ragged last stage lands on this CTA's own barrier:
                         // its tail is zeroed before the leader hears of it.
+                        int here = L::kBlocks;
                         if (w.tail != 0 && kb == w.blocks - 1) {
-                            ptx::mbar_arrive_expect_tx(&bar.landed[ring.stage], L::kABytes + b_bytes);
+                            here = (w.tail + 63) / 64;
+                            ptx::mbar_arrive_expect_tx(&bar.landed[ring.stage], here * (L::kABlock + b_bytes));
                             if (leader) ptx::mbar_arrive(&bar.full[ring.stage]);
                             full = ptx::mapa_shared(ptx::smem_addr(&bar.landed[ring.stage]), rank);
                         } else if (leader) {
-                            ptx::mbar_arrive_expect_tx(&bar.full[ring.stage], 2 * (L::kABytes + b_bytes));
+                            ptx::mbar_arrive_expect_tx(&bar.full[ring.stage], 2 * here * (L::kABlock + b_bytes));
                         }
-                        const int t0 = w.t0 + kb * 64;
-                        for (int i = 0; i < 2; ++i) ptx::tma_load_2d_pair(sa + i * 8192, &map_a, full, a0 + 64 * i, t0);
-                        for (int i = 0; i < boxes; ++i)
-                            ptx::tma_load_2d_pair(sb + i * 8192, &map_b64, full, b0 + 64 * i, t0);
+                        for (int h = 0; h < here; ++h) {
+                            const int t0 = w.t0 + kb * L::kBK + h * 64;
+                            for (int i = 0; i < 2; ++i)
+                                ptx::tma_load_2d_pair(sa + h * L::kABlock + i * 8192, &map_a, full, a0 + 64 * i, t0);
+                            for (int i = 0; i < boxes; ++i)
+                                ptx::tma_load_2d_pair(sb + h * L::kBBlock + i * 8192, &map_b64, full, b0 + 64 * i, t0);
+                        }
                     } else {
-                        if (leader) ptx::mbar_arrive_expect_tx(&bar.full[ring.stage], 2 * (L::kABytes + b_bytes));
+                        if (leader) ptx::mbar_arrive_expect_tx(&bar.full[ring.stage], 2 * L::kBlocks * (L::kABlock + b_bytes));
                         for (int h = 0; h < L::kBlocks; ++h) {
                             const int k0 = L::kMx ? kb * 128 : kb * L::kBK + h * 64;  // MXFP4 maps count bytes
                             if constexpr (L::kAMn) {
@@ -277,7 +288,7 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                 }
             }
             // The leader's full barriers count both CTAs' copies; none may be
-            // in flight when a CTA leaves.  (A ragged block's are waited for by
+            // in flight when a CTA leaves.  (A ragged stage's are waited for by
             // the warp that zeroes its tail.)
             for (int s = 0; s < S; ++s) {
                 if (leader && (issued & (1u << s)) &&
@@ -403,9 +414,9 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                     __syncwarp();
                     if (lane == 0 && n0 < p.n && col < p.k) {
                         if (p.accumulate)
-                            ptx::tma_add_3d(&map_c, staging, col, n0, w.e);
+                            ptx::tma_add_3d(&map_c, staging, col, n0, p.first_group + w.e);
                         else
-                            ptx::tma_store_3d_hint(&map_c, staging, col, n0, w.e, policy);
+                            ptx::tma_store_3d_hint(&map_c, staging, col, n0, p.first_group + w.e, policy);
                         ptx::bulk_commit_group();
                     }
                 };
@@ -589,14 +600,17 @@ __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
                     break;
                 }
                 landed_phase ^= 1u << ring.stage;
-                // Rows tail .. next multiple of 16 of every box: 128 bytes each
-                // whatever the swizzle, which permutes within a row.
+                // Rows tail .. next multiple of 16 of every box of their block:
+                // 128 bytes each whatever the swizzle, which permutes within a
+                // row.  (A multiple of 16 needs none.)
+                const int block = w.tail / 64, first = w.tail % 64, count = round_up(w.tail, 16) - w.tail;
                 uint8_t* stage = smem + ring.stage * L::kStageBytes;
                 const int boxes = 2 + (w.width / 2 + 63) / 64;
-                const int first = w.tail, count = round_up(w.tail, 16) - w.tail;
                 for (int i = lane; i < boxes * count * 8; i += 32) {
                     const int box = i / (count * 8), at = i % (count * 8);
-                    *reinterpret_cast<uint4*>(stage + box * 8192 + first * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+                    uint8_t* base = box < 2 ? stage + block * L::kABlock + box * 8192
+                                            : stage + L::kABytes + block * L::kBBlock + (box - 2) * 8192;
+                    *reinterpret_cast<uint4*>(base + first * 128 + at * 16) = make_uint4(0, 0, 0, 0);
                 }
                 // Read by this CTA's own tensor core: see the scales' arrivals.
                 ptx::fence_proxy_async_smem();
@@ -642,7 +656,7 @@ int launch(const CUtensorMap& a, const CUtensorMap (&b)[3], const CUtensorMap& c
         std::lock_guard<std::mutex> lock(mu);
         if (!configured[device]) {
             if (cudaFuncSetAttribute(grouped_pair_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     L::smem_bytes(KMCTS_MAX_GROUPS)) != cudaSuccess)
+                                     L::smem_bytes(L::kMaxGroups)) != cudaSuccess)
                 return KMCTS_EGEMM;
             configured[device] = true;
         }
@@ -724,7 +738,13 @@ int launch_wgrad_pair(const WgradArgs& g, uint64_t limit_ns, cudaStream_t stream
     p.strip = Divisor::of(8 * ((g.k + 255) / 256));
     p.per_group = Divisor::of(static_cast<uint32_t>(tiles / g.groups));
     p.stream_out = static_cast<int64_t>(g.groups) * g.n * g.k * (g.fp32 ? 4 : 2) > 63LL << 20;  // L2 is 126 MB
-    return launch<Kind::kWgrad>(a, b, c, p, tiles, stream);
+    constexpr int most = Pair<Kind::kWgrad>::kMaxGroups;
+    for (; p.first_group < g.groups; p.first_group += most) {
+        p.groups = g.groups - p.first_group < most ? g.groups - p.first_group : most;
+        const int rc = launch<Kind::kWgrad>(a, b, c, p, static_cast<int64_t>(p.groups) * p.per_group.d, stream);
+        if (rc != KMCTS_OK) return rc;
+    }
+    return KMCTS_OK;
 }
 
 }  // namespace grouped
