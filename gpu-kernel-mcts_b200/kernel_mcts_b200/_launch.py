@@ -125,6 +125,15 @@ def caller_stream(index: int, stream: torch.cuda.Stream | None) -> torch.cuda.St
     return current if current != stream else None
 
 
+def use_on(stream: torch.cuda.Stream | None, caller: torch.cuda.Stream | None, *tensors: torch.Tensor | None) -> None:
+    """Marks the caller's tensors as used by the side stream of a call, so
+    that memory they free before the call is done waits for it."""
+    if caller is not None:
+        for tensor in tensors:
+            if tensor is not None:
+                tensor.record_stream(stream)
+
+
 def share_result(result: torch.Tensor, caller: torch.cuda.Stream | None) -> torch.Tensor:
     """Marks a tensor allocated on a side stream as used by the stream the
     caller works on, so that its memory is not handed out again too early."""

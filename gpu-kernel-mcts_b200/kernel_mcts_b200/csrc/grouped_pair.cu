@@ -17,9 +17,17 @@
 //
 // Roles per CTA: warp 0 TMA producer; warp 1 MMA (the pair's leader issues);
 // warps 2-9 epilogue; MXFP4 adds four warps that fetch scales and one that
-// issues their copies into TMEM, the gradient one that zeroes tails.  Every CTA reads the groups' ends itself and walks
-// the tiles round-robin; nothing is decided on the host.  Every wait is
-// bounded.
+// issues their copies into TMEM, the gradient one that zeroes tails.  Every CTA
+// reads the groups' ends itself and walks the tiles round-robin; nothing is
+// decided on the host.  Every wait is bounded.
+//
+// Bounds and layout, measured on B200 (bursts): forward products run at 1.2 to
+// 1.5 PFLOP/s, the tensor pipe busy 78% of the time, held back by operands
+// from L2 (10 TB/s into the SMs) and by tiles that do not share out evenly over
+// 74 pairs; gradients at 1.1 to 1.4, where short contractions are bound by
+// writing the gradient; MXFP4 at 4.0, bound by L2 likewise (each tile moves 448
+// rows of operands for 256 x 192 outputs).  Longest-tile-first orders would
+// gain 2 to 3% on skewed groups by simulation and are left out.
 #include <mutex>
 
 #include "grouped_tiles.cuh"
@@ -145,8 +153,7 @@ template <Kind KIND>
 __global__ void __launch_bounds__(Pair<KIND>::kThreads, 1)
     grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b128,
                         const __grid_constant__ CUtensorMap map_b64, const __grid_constant__ CUtensorMap map_b32,
-                        const __grid_constant__ CUtensorMap map_c,
-                        const __grid_constant__ PairParams p) {
+                        const __grid_constant__ CUtensorMap map_c, const __grid_constant__ PairParams p) {
     using L = Pair<KIND>;
     constexpr int S = L::kStages;
     extern __shared__ uint8_t smem_raw[];

@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
                 ok = ptx::mbar_wait(&tmem_full[acc], (local >> 1) & 1, p.limit_ns, abort);
                 ++local;
             }
-            if (ok && seen > 0) ok = ptx::mbar_wait(&freed[quarter], (seen - 1) & 1, p.limit_ns, abort);
+            if (ok && seen > 0) ok = ptx::mbar_wait_cluster(&freed[quarter], (seen - 1) & 1, p.limit_ns, abort);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) record_failure(p.status, abort, kRoleEpilogue);
                 break;
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
             // Four parts of width x 32 values come here, whatever S is.
             if (threadIdx.x == 64) ptx::mbar_arrive_expect_tx(arrived, static_cast<uint32_t>(w.width * 512));
             // The parts of this CTA's quarters: the four warps share the tokens.
-            ok = __all_sync(0xffffffffu, ptx::mbar_wait(arrived, seen & 1, p.limit_ns, abort));
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait_cluster(arrived, seen & 1, p.limit_ns, abort));
             if (!ok) {
                 if (lane == 0) record_failure(p.status, abort, kRoleEpilogue);
                 break;

@@ -71,6 +71,7 @@ def grouped_gemm(
     status_ptr = _launch.status_pointer(status, device)
     kernel_id = kernel_code(kernel)
     caller = _launch.caller_stream(device, stream)
+    _launch.use_on(stream, caller, x, w, ends, out, status)
     with _launch.on_device(device, stream):
         if out is None:
             out = _launch.share_result(x.new_empty((rows, n)), caller)
@@ -104,8 +105,8 @@ def grouped_gemm_wgrad(
 
     The result is ``dtype`` (bfloat16 by default, or float32) or ``out``'s type.
     ``accumulate`` adds to a float32 ``out``, as for a main gradient kept over
-    several micro-batches; an empty group then leaves its part as it was, and
-    is zeros otherwise.
+    several micro-batches (sums below ``2^-126`` become zero); an empty group
+    then leaves its part as it was, and is zeros otherwise.
     """
     device = dy.get_device()
     (rows, n), _, lddy = _launch.rows_of("dy", dy, 2, _BF16, device, 8)
@@ -123,6 +124,7 @@ def grouped_gemm_wgrad(
     status_ptr = _launch.status_pointer(status, device)
     kernel_id = kernel_code(kernel, _GRADIENT_KERNELS)
     caller = _launch.caller_stream(device, stream)
+    _launch.use_on(stream, caller, dy, x, ends, out, status)
     with _launch.on_device(device, stream):
         if out is None:
             out = _launch.share_result(x.new_empty((groups, n, k), dtype=dtype), caller)

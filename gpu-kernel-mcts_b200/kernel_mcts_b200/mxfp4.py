@@ -84,6 +84,7 @@ def mxfp4_quantize(
     (rows, k), _, ldx = _launch.rows_of("x", flat, 2, _TYPE_TUPLE, device, BLOCK)
     _launch.check_sizes(k)
     caller = _launch.caller_stream(device, stream)
+    _launch.use_on(stream, caller, x, *(out or ()))
     with _launch.on_device(device, stream):
         if out is None:
             lead = shape[:-1]
@@ -124,6 +125,7 @@ def mxfp4_dequantize(
     if dtype not in _TYPES:
         raise TypeError(f"values must be bfloat16, float16 or float32, got {dtype}")
     caller = _launch.caller_stream(device, stream)
+    _launch.use_on(stream, caller, *q, out)
     with _launch.on_device(device, stream):
         if out is None:
             flat = out = _launch.share_result(codes.new_empty(q.shape, dtype=dtype), caller)
@@ -155,7 +157,9 @@ def mxfp4_gemm(
 
     ``a`` is ``[rows, K]``.  Without ``ends``, ``b`` is ``[N, K]``; with
     ``ends``, ``b`` is ``[groups, N, K]`` and each row of ``a`` meets its own
-    group's weight, as in :func:`kernel_mcts_b200.grouped.grouped_gemm`.
+    group's weight; groups, ``out`` and ``kernel`` are as in
+    :func:`kernel_mcts_b200.grouped.grouped_gemm`.  Code rows that do not start
+    on 16 bytes take the CUDA-core kernel; scales may lie at any address.
     """
     device = a[0].get_device()
     (rows, half), _, lda, _, ldas = _pair_rows("a", a, 2, device)
@@ -174,6 +178,7 @@ def mxfp4_gemm(
     status_ptr = _launch.status_pointer(status, device)
     kernel_id = kernel_code(kernel)
     caller = _launch.caller_stream(device, stream)
+    _launch.use_on(stream, caller, *a, *b, ends, out, status)
     with _launch.on_device(device, stream):
         if out is None:
             out = _launch.share_result(a[1].new_empty((rows, n), dtype=torch.bfloat16), caller)
