@@ -278,8 +278,15 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
                 ++local;
             }
             if (ok && seen > 0) ok = ptx::mbar_wait_cluster(&freed[quarter], (seen - 1) & 1, p.limit_ns, abort);
-            if (!__all_sync(0xffffffffu, ok)) {
+            // Four parts of width x 32 values come here, whatever S is.  Their
+            // stores are asynchronous: a CTA that gives up still waits
+            // (bounded) for the other CTAs' before it leaves.
+            const uint32_t part_bytes = static_cast<uint32_t>(w.width * 512);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
                 if (lane == 0) record_failure(p.status, abort, kRoleEpilogue);
+                if (threadIdx.x == 64) ptx::mbar_arrive_expect_tx(arrived, part_bytes);
+                ptx::mbar_wait_cluster(arrived, seen & 1, drain_limit(p.limit_ns), no_abort);
                 break;
             }
             ptx::tc_fence_after();
@@ -307,10 +314,9 @@ __global__ void __launch_bounds__(Split<KIND>::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&tmem_empty[acc]);
             }
-            // Four parts of width x 32 values come here, whatever S is.
-            if (threadIdx.x == 64) ptx::mbar_arrive_expect_tx(arrived, static_cast<uint32_t>(w.width * 512));
+            if (threadIdx.x == 64) ptx::mbar_arrive_expect_tx(arrived, part_bytes);
             // The parts of this CTA's quarters: the four warps share the tokens.
-            ok = __all_sync(0xffffffffu, ptx::mbar_wait_cluster(arrived, seen & 1, p.limit_ns, abort));
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait_cluster(arrived, seen & 1, drain_limit(p.limit_ns), no_abort));
             if (!ok) {
                 if (lane == 0) record_failure(p.status, abort, kRoleEpilogue);
                 break;
