@@ -177,7 +177,9 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *, w_la
     """Differentiable ``grouped_gemm(x, w, ends, w_layout=w_layout)``.
 
     The gradients of ``x`` and ``w`` are bfloat16; ``x``'s is zero in rows
-    behind the last group.  Once differentiable."""
+    behind the last group.  Once differentiable.  As with any torch function, a
+    backward pass may be captured into a CUDA graph only while no autograd
+    graph of the same leaves from outside the capture is alive."""
     return _GroupedLinear.apply(x, w, ends, layout_code(w_layout))
 
 

@@ -46,6 +46,39 @@ def test_row_stride_of_one_row_is_its_length():
         stride(torch.zeros(13).expand(4, 13))
 
 
+def test_calls_run_on_the_operands_device(monkeypatch):
+    """The context of a call sets the operands' device where it is not the
+    current one, and refuses a stream of another device."""
+    entered = []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            entered.append(self.index)
+
+        def __exit__(self, *exc):
+            entered.append("left")
+
+    monkeypatch.setattr(_launch, "_current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    with _launch.on_device(0, None):
+        assert entered == []
+    with _launch.on_device(1, None):
+        assert entered == [1]
+    assert entered == [1, "left"]
+    stream = type("Stream", (), {"device": torch.device("cuda", 0)})()
+    with pytest.raises(ValueError, match="stream is on"):
+        _launch.on_device(1, stream)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    with pytest.raises(ValueError, match="at most"):
+        _launch.check_sizes(8, 2 ** 31)
+    assert _forward(rows=2 ** 31 - 1) == _native.KMCTS_EINVAL
+
+
 def _forward(**change):
     args = dict(x=P, ldx=64, w=P, w_stride=64 * 32, ldw=64, layout=0, y=P, ldy=32, ends=P, groups=2, rows=4, n=32, k=64,
                 flags=0, kernel=0)

@@ -299,6 +299,37 @@ def test_step_as_a_graph(cuda_device):
     assert torch.equal(gw, wgrad64(dy, x.detach(), counts)[0].to(torch.bfloat16))
 
 
+def test_graph_with_copies_and_a_side_stream(cuda_device):
+    """Calls captured behind a fill, a copy and a join with another stream,
+    on which a call of its own was captured."""
+    counts, n, k = [40, 0, 30], 128, 256
+    x, w = integers(70, k, seed=1), integers(3, n, k, seed=2)
+    ends, source = torch.zeros(3, dtype=torch.int32, device="cuda"), ends_of(counts)
+    out = torch.ones(80, n, dtype=torch.bfloat16, device="cuda")
+    side = torch.cuda.Stream()
+    ref = forward64(x, w, counts, "col")[0].to(torch.bfloat16)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ends.copy_(source)
+        out.zero_()
+        grouped.grouped_gemm(x, w, ends, out[:70])
+        side.wait_stream(torch.cuda.current_stream())
+        dw = grouped.grouped_gemm_wgrad(out[:70], x, ends, stream=side, dtype=torch.float32)
+        y = grouped.grouped_gemm(out[:70], w, ends, w_layout="row")
+        torch.cuda.current_stream().wait_stream(side)
+        total = y.float().sum() + dw.sum()
+    for _ in range(2):
+        ends.fill_(-1)
+        out.fill_(5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:70], ref) and (out[70:] == 0).all()
+        assert within(dw, *wgrad64(ref, x, counts), 40, 2.0 ** -24)
+        y64, mag = forward64(ref, w, counts, "row")
+        assert within(y, y64, mag, n, 2.0 ** -8) and total.isfinite()
+
+
 def test_two_streams_at_once(cuda_device):
     """Calls that overlap on the GPU share nothing."""
     counts, n, k = [700, 30, 300], 512, 1024
