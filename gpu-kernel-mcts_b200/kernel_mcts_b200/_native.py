@@ -11,7 +11,7 @@ import ctypes
 import threading
 from pathlib import Path
 
-from .build import LIBRARY
+from .build import LIBRARY, TORCH_CALLS
 
 KMCTS_OK = 0
 KMCTS_EHANDLE = 1
@@ -263,6 +263,34 @@ def load() -> ctypes.CDLL:
             getattr(lib, name).restype = i32
         _lib = lib
         return lib
+
+
+_calls = None
+
+
+def load_torch_calls():
+    """Loads (once) and returns the module of expert-layer calls on torch
+    tensors, which is built against the library of :func:`load`."""
+    global _calls
+    load()
+    with _lock:
+        if _calls is None:
+            import importlib.util
+
+            import torch  # noqa: F401  (its libraries are the module's)
+
+            if not TORCH_CALLS.exists():
+                raise NativeLibraryError(
+                    f"{TORCH_CALLS} is not built; run kernel_mcts_b200.build.build_all() (g++, torch headers)"
+                )
+            spec = importlib.util.spec_from_file_location("kmcts_torch_calls", TORCH_CALLS)
+            try:
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+            except ImportError as error:
+                raise NativeLibraryError(f"cannot load {TORCH_CALLS}: {error}") from error
+            _calls = module
+        return _calls
 
 
 def default_config() -> GemmConfig:

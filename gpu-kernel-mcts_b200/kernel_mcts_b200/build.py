@@ -3,6 +3,7 @@
 Outputs (git-ignored, shipped with the source tree):
   _lib/libkmcts_gemm_sm100.so   the C-ABI library (include/kmcts_gemm.h, kmcts_grouped.h)
   _lib/kmcts_bf16_eval          the evaluation harness executable built on it
+  _lib/kmcts_torch_calls.so     the expert-layer calls on torch tensors (host code)
 
 Run as ``python -m kernel_mcts_b200.build`` (with gpu-kernel-mcts_b200/ on
 sys.path) or call :func:`build_all`.  Rebuilds only what is older than its
@@ -16,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -27,6 +29,7 @@ OBJ_DIR = LIB_DIR / "obj"
 
 LIBRARY = LIB_DIR / "libkmcts_gemm_sm100.so"
 HARNESS = LIB_DIR / "kmcts_bf16_eval"
+TORCH_CALLS = LIB_DIR / "kmcts_torch_calls.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = ["-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}"]
@@ -119,9 +122,38 @@ def build_harness(verbose: bool = False) -> Path:
     return HARNESS
 
 
+def build_torch_calls(verbose: bool = False) -> Path:
+    """The torch-facing calls: host code only, against this interpreter's torch."""
+    import importlib.util
+
+    lib = build_library(verbose)
+    src = CSRC / "torch_calls.cpp"
+    headers = (INCLUDE / "kmcts_grouped.h", INCLUDE / "kmcts_gemm.h")
+    if not _stale(TORCH_CALLS, [src, *headers, Path(__file__)]):
+        return TORCH_CALLS
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        raise RuntimeError("torch not found; the expert-layer calls are built against its headers")
+    torch_dir = Path(spec.origin).parent
+    includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
+                Path(sysconfig.get_paths()["include"]), Path(nvcc()).resolve().parent.parent / "include"]
+    cmd = [
+        shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{INCLUDE}",
+        *(arg for path in includes for arg in ("-isystem", str(path))), str(src), "-o", str(TORCH_CALLS),
+        f"-L{LIB_DIR}", f"-l{lib.stem.removeprefix('lib')}", f"-L{torch_dir / 'lib'}",
+        *(f"-l{name}" for name in ("c10", "c10_cuda", "torch", "torch_cpu", "torch_cuda", "torch_python")),
+        "-Wl,-rpath,$ORIGIN",
+    ]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    _run(cmd)
+    return TORCH_CALLS
+
+
 def build_all(verbose: bool = False) -> None:
     build_library(verbose)
     build_harness(verbose)
+    build_torch_calls(verbose)
 
 
 if __name__ == "__main__":

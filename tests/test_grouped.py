@@ -36,46 +36,52 @@ def test_cpu_tensors_and_other_types_are_refused():
         mxfp4.mxfp4_gemm(q, q)
 
 
-def test_row_stride_of_one_row_is_its_length():
-    def stride(t):
-        return _launch.row_stride("x", t.shape, t.stride(), 0, 8)
-
-    assert stride(torch.zeros(1, 13)) == 16
-    assert stride(torch.zeros(4, 40)[:, :13]) == 40
-    with pytest.raises(ValueError, match="overlapping"):
-        stride(torch.zeros(13).expand(4, 13))
+class FakeStream:
+    def __init__(self, index):
+        self.device = torch.device("cuda", index)
 
 
-def test_calls_run_on_the_operands_device(monkeypatch):
-    """The context of a call sets the operands' device where it is not the
-    current one, and refuses a stream of another device."""
-    entered = []
+class FakeTensor:
+    def __init__(self, index):
+        self.index, self.used_by = index, []
 
-    class Device:
-        def __init__(self, index):
-            self.index = index
+    def get_device(self):
+        return self.index
+
+    def record_stream(self, stream):
+        self.used_by.append(stream)
+
+
+def test_a_side_stream_runs_the_call_and_marks_every_tensor(monkeypatch):
+    here, side = FakeStream(1), FakeStream(1)
+    current = [here]
+
+    class OnStream:
+        def __init__(self, stream):
+            self.stream = stream
 
         def __enter__(self):
-            entered.append(self.index)
+            current.append(self.stream)
 
         def __exit__(self, *exc):
-            entered.append("left")
+            current.pop()
 
-    monkeypatch.setattr(_launch, "_current_device", lambda: 0)
-    monkeypatch.setattr(torch.cuda, "device", Device)
-    with _launch.on_device(0, None):
-        assert entered == []
-    with _launch.on_device(1, None):
-        assert entered == [1]
-    assert entered == [1, "left"]
-    stream = type("Stream", (), {"device": torch.device("cuda", 0)})()
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: current[-1])
+    monkeypatch.setattr(torch.cuda, "stream", OnStream)
+    x, out, result = FakeTensor(1), FakeTensor(1), (FakeTensor(1), FakeTensor(1))
+
+    def call(a, b):
+        assert (a, b) == (x, 3) and current[-1] is side
+        return result
+
+    assert _launch.run_on(side, (x, None, out), call, x, 3) is result
+    assert x.used_by == out.used_by == [side] and [t.used_by for t in result] == [[here], [here]]
+    assert _launch.run_on(here, (x,), lambda: current[-1]) is here and x.used_by == [side]
     with pytest.raises(ValueError, match="stream is on"):
-        _launch.on_device(1, stream)
+        _launch.run_on(FakeStream(0), (x,), call)
 
 
 def test_sizes_beyond_32_bits_are_refused():
-    with pytest.raises(ValueError, match="at most"):
-        _launch.check_sizes(8, 2 ** 31)
     assert _forward(rows=2 ** 31 - 1) == _native.KMCTS_EINVAL
 
 

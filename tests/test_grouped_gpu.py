@@ -168,6 +168,15 @@ def test_strided_operands(cuda_device, kernel, layout):
 
 
 @pytest.mark.parametrize("kernel", KERNELS)
+def test_one_row_of_any_stride(cuda_device, kernel):
+    x = integers(16, 1, seed=1).T  # [1, 16] with strides (1, 1)
+    w = integers(1, 24, 16, seed=2)
+    out = torch.zeros(24, dtype=torch.bfloat16, device="cuda").as_strided((1, 24), (1, 1))
+    checked(grouped.grouped_gemm, x, w, ends_of([1]), out, kernel=kernel)
+    assert torch.equal(out, forward64(x, w, [1], "col")[0].to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
 def test_ends_out_of_order_or_range_are_clamped(cuda_device, kernel):
     n, k = 64, 64
     x, w = integers(200, k, seed=1), integers(5, n, k, seed=2)
