@@ -400,10 +400,12 @@ PYBIND11_MODULE(kmcts_torch_calls, m) {
             PyErr_SetObject(error.ptr(), error(failure.code, failure.call).ptr());
         }
     });
-    m.def("grouped_gemm", &grouped_gemm);
-    m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad);
-    m.def("grouped_linear", &grouped_linear);
-    m.def("mxfp4_quantize", &mxfp4_quantize);
-    m.def("mxfp4_dequantize", &mxfp4_dequantize);
-    m.def("mxfp4_gemm", &mxfp4_gemm);
+    // A launch waits while the device's queue is full: other threads go on meanwhile.
+    const py::call_guard<py::gil_scoped_release> unlocked;
+    m.def("grouped_gemm", &grouped_gemm, unlocked);
+    m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, unlocked);
+    m.def("grouped_linear", &grouped_linear, unlocked);
+    m.def("mxfp4_quantize", &mxfp4_quantize, unlocked);
+    m.def("mxfp4_dequantize", &mxfp4_dequantize, unlocked);
+    m.def("mxfp4_gemm", &mxfp4_gemm, unlocked);
 }

@@ -11,6 +11,10 @@ Bars:
 
 from __future__ import annotations
 
+import time
+from concurrent.futures import ThreadPoolExecutor
+from threading import Thread
+
 import pytest
 import torch
 
@@ -502,3 +506,48 @@ def test_refusals(cuda_device):
     assert grouped.grouped_gemm(x[:0], w, ends).shape == (0, 8)
     assert (grouped.grouped_gemm(x[:, :0], w[:, :, :0], ends) == 0).all()
     assert (grouped.grouped_gemm_wgrad(x[:0], x[:0], ends) == 0).all()
+
+
+def test_threads_on_their_own_streams():
+    counts = [5, 0, 130, 9]
+    x, w, ends = integers(sum(counts), 136), integers(4, 200, 136, seed=1), ends_of(counts)
+    want = forward64(x, w, counts, "col")[0].to(torch.bfloat16)
+    torch.cuda.synchronize()
+
+    def work(_):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            ys = [grouped.grouped_gemm(x, w, ends) for _ in range(50)]
+        stream.synchronize()
+        return all(torch.equal(y, want) for y in ys)
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
+
+
+def test_other_threads_run_while_a_launch_waits():
+    # The device sleeps while one thread fills its launch queue and waits; this
+    # thread must go on.  Its longest pause stays below half of the sleep.
+    x, w, ends = integers(4, 64), integers(1, 64, 64, seed=1), ends_of([4])
+    out = grouped.grouped_gemm(x, w, ends)
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    torch.cuda.synchronize()
+    begin.record()
+    torch.cuda._sleep(2_000_000_000)
+    end.record()
+
+    def fill():
+        for _ in range(4000):
+            grouped.grouped_gemm(x, w, ends, out)
+
+    # The clock starts first: the queue is full within one interpreter switch interval.
+    thread = Thread(target=fill)
+    pause, last = 0.0, time.perf_counter()
+    thread.start()
+    while thread.is_alive():
+        time.sleep(0.001)
+        now = time.perf_counter()
+        pause, last = max(pause, now - last), now
+    thread.join()
+    torch.cuda.synchronize()
+    assert pause < begin.elapsed_time(end) / 1000 / 2
