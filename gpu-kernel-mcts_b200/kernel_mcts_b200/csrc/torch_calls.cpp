@@ -286,6 +286,7 @@ PairStrides check_pair(const char* name, const Tensor& codes, const Tensor& scal
 
 std::tuple<Tensor, Tensor> mxfp4_quantize(const Tensor& x, const std::optional<Tensor>& out_codes,
                                           const std::optional<Tensor>& out_scales) {
+    if (out_codes.has_value() != out_scales.has_value()) throw py::value_error("out must hold both codes and scales");
     if (x.dim() < 1 || x.size(-1) % kBlock != 0)
         throw py::value_error(text("x must have a last dimension that is a multiple of ", kBlock, ", got shape ",
                                    shape_text(x.sizes())));

@@ -141,3 +141,10 @@ def test_c_mxfp4_gemm_refuses(change):
                 ldy=16, ends=P, groups=2, rows=4, n=16, k=64, flags=0, kernel=0)
     args.update(change)
     assert _native.load().kmcts_mxfp4_gemm(*args.values(), None, None) == _native.KMCTS_EINVAL
+
+
+@pytest.mark.parametrize("missing", ["codes", "scales"])
+def test_mxfp4_results_come_in_pairs(missing):
+    out = mxfp4.MXFP4Tensor(torch.zeros(2, 16, dtype=torch.uint8), torch.zeros(2, 1, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="codes and scales"):
+        mxfp4.mxfp4_quantize(torch.zeros(2, 32), out._replace(**{missing: None}))
