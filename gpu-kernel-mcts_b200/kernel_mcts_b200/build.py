@@ -38,7 +38,7 @@ LIBRARY_SOURCES = ("gemm_tcgen05.cu", "gemm_tcgen05_pair.cu", "gemm_tcgen05_stre
                    "capi.cu", "ipc.cu", "selftest.cu", "workspace.cu", "host_gemm.cu")
 GROUPED_SOURCES = ("grouped_api.cu", "grouped_pair.cu", "grouped_split.cu", "grouped_simt.cu", "mxfp4_quantize.cu")
 HEADERS = ("ptx_sm100.cuh", "gemm_common.cuh", "kmcts_internal.h")
-GROUPED_HEADERS = ("grouped_common.cuh", "grouped_internal.h", "grouped_tiles.cuh", "ptx_grouped.cuh")
+GROUPED_HEADERS = ("grid_walk.h", "grouped_common.cuh", "grouped_internal.h", "grouped_tiles.cuh", "ptx_grouped.cuh")
 
 
 def nvcc() -> str:

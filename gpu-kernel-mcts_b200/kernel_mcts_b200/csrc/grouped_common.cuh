@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "grid_walk.h"
 #include "grouped_internal.h"
 
 namespace kmcts {
@@ -109,8 +110,8 @@ __device__ __forceinline__ int group_of_tile(const GroupTable& table, int t, int
 // Zeroes the rows of Y behind the last group, spread over the whole grid.
 __device__ __forceinline__ void zero_rest_rows(__nv_bfloat16* y, int64_t ldy, int first, int rows, int n, int block,
                                                int blocks) {
-    for (int r = first + block; r < rows; r += blocks)
-        for (int c = threadIdx.x; c < n; c += blockDim.x) y[static_cast<int64_t>(r) * ldy + c] = __float2bfloat16(0.0f);
+    for (GridWalk r(first, rows, block, blocks); r.more(); r.next())
+        for (int c = threadIdx.x; c < n; c += blockDim.x) y[r.at * ldy + c] = __float2bfloat16(0.0f);
 }
 
 // E8M0: 2^(s - 127); 0 is the subnormal 2^-127, 255 is NaN.

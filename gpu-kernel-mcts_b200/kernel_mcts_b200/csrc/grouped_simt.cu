@@ -55,7 +55,8 @@ __global__ void __launch_bounds__(kThreads) grouped_forward_simt(ForwardArgs p) 
     __syncthreads();
     auto* y = static_cast<__nv_bfloat16*>(p.y);
     int group = 0;
-    for (int t = blockIdx.x; t < table.tiles(); t += gridDim.x) {
+    for (GridWalk walk(0, table.tiles(), blockIdx.x, gridDim.x); walk.more(); walk.next()) {
+        const int t = static_cast<int>(walk.at);
         const int e = group_of_tile(table, t, group);
         const int in_group = t - table.tile[e];
         const int64_t row0 = table.row[e] + in_group / tiles_n * kTile;
@@ -104,7 +105,8 @@ __global__ void __launch_bounds__(kThreads) grouped_wgrad_simt(WgradArgs p) {
     const int per_group = (p.n + kTile - 1) / kTile * tiles_k;
     if (threadIdx.x < 32) build_group_table(table, p.ends, p.rows, [&](int) { return per_group; });
     __syncthreads();
-    for (int t = blockIdx.x; t < table.tiles(); t += gridDim.x) {
+    for (GridWalk walk(0, table.tiles(), blockIdx.x, gridDim.x); walk.more(); walk.next()) {
+        const int t = static_cast<int>(walk.at);
         const int e = t / per_group;
         const int n0 = t % per_group / tiles_k * kTile, k0 = t % tiles_k * kTile;
         const int rows = min(kTile, p.n - n0), cols = min(kTile, p.k - k0);
