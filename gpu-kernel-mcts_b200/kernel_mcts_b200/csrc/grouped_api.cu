@@ -75,6 +75,18 @@ bool bad_sizes(int groups, int rows, int n, int k) {
            groups > KMCTS_MAX_GROUPS;
 }
 
+// How long a wait of a launch may last: the library's limit, and ten
+// microseconds for each stage that one CTA walks through.  Epilogues and the
+// gradient's tail warps sleep through the whole contraction of a tile (the tail
+// warps through tiles without a tail, too), which takes 0.3 to 1.2 us a stage:
+// with the limit alone, contractions of more than about 2 s were given up.  Ten
+// minutes are more than any product takes whose operands fit in memory.
+uint64_t wait_limit(int64_t stages) {
+    constexpr uint64_t most = 600000000000ull;
+    const uint64_t limit = gemm::kDefaultWaitNs + 10000ull * static_cast<uint64_t>(stages);
+    return limit < most ? limit : most;
+}
+
 // Whether the few-rows kernel should take a product, and how many CTAs share
 // one of its tiles (128 weight rows x 64 tokens; how many there are is known
 // up to where the groups end).  GPU time on B200 with operands read from HBM,
@@ -111,8 +123,9 @@ int forward(const ForwardArgs& a, Operand kind, int kernel, cudaStream_t stream,
         if (!status) return KMCTS_EHANDLE;
         const FewRows few = few_rows(a);
         const bool split = kernel == KMCTS_KERNEL_GROUPED_SPLIT || (few.better && kernel != KMCTS_KERNEL_GROUPED_PAIR);
-        const int rc = split ? launch_forward_split(a, kind, few.splits, gemm::kDefaultWaitNs, stream, status)
-                             : launch_forward_pair(a, kind, gemm::kDefaultWaitNs, stream, status);
+        const uint64_t limit = wait_limit(a.k / (kind == Operand::kMxfp4 ? 256 : 64) + 1);
+        const int rc = split ? launch_forward_split(a, kind, few.splits, limit, stream, status)
+                             : launch_forward_pair(a, kind, limit, stream, status);
         if (rc != KMCTS_ENOTSUP || kernel != KMCTS_KERNEL_AUTO) return rc;
     }
     return launch_forward_simt(a, kind, stream);
@@ -158,7 +171,10 @@ int kmcts_bf16_grouped_wgrad(const void* dY, int64_t lddy, const void* X, int64_
     if (kernel != KMCTS_KERNEL_SIMT && rows > 0) {
         int* status = device_status ? device_status : default_status_ptr();
         if (!status) return KMCTS_EHANDLE;
-        const int rc = launch_wgrad_pair(a, gemm::kDefaultWaitNs, s, status);
+        // A pair takes every 74th tile of each group in turn.
+        const int64_t tiles = ((N + 255LL) / 256) * ((K + 255LL) / 256), pairs = multiprocessor_count() / 2;
+        const int64_t stages = (rows / 128 + static_cast<int64_t>(groups)) * ((tiles + pairs - 1) / pairs);
+        const int rc = launch_wgrad_pair(a, wait_limit(stages), s, status);
         if (rc != KMCTS_ENOTSUP || kernel != KMCTS_KERNEL_AUTO) return rc;
     }
     return launch_wgrad_simt(a, s);
