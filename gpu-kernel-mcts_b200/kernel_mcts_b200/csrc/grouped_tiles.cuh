@@ -104,13 +104,13 @@ __device__ __forceinline__ void load_scale_words(const uint8_t* row, int first, 
         if (16 * c >= bytes) break;
         const uint8_t* src = base + 16 * c;
         if (src >= span.begin && src + 16 <= span.end) {
-            out[c] = __ldg(reinterpret_cast<const uint4*>(src));
+            out[c] = *reinterpret_cast<const uint4*>(src);
         } else {
             uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int b = 0; b < 16; ++b)
                 if (src + b >= span.begin && src + b < span.end)
-                    w[b / 4] |= static_cast<uint32_t>(__ldg(src + b)) << (8 * (b % 4));
+                    w[b / 4] |= static_cast<uint32_t>(src[b]) << (8 * (b % 4));
             out[c] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }

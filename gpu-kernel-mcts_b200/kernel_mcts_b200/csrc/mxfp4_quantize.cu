@@ -116,9 +116,8 @@ __device__ __forceinline__ uint32_t largest_bits(const Chunk<TYPE> (&in)[kHeld<T
 
 template <int TYPE, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads)
-    mxfp4_quantize_kernel(const typename Element<TYPE>::type* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
-                          int64_t ldc, uint8_t* __restrict__ scales, int64_t lds, int64_t rows, unsigned per_row,
-                          unsigned rows_per_block) {
+    mxfp4_quantize_kernel(const typename Element<TYPE>::type* x, int64_t ldx, uint8_t* codes, int64_t ldc,
+                          uint8_t* scales, int64_t lds, int64_t rows, unsigned per_row, unsigned rows_per_block) {
     ptx::let_next_grid_start();
     ptx::wait_for_earlier_grids();
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;
@@ -172,9 +171,9 @@ constexpr int kBatch = 4;
 
 template <int TYPE, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads)
-    mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const uint8_t* __restrict__ scales,
-                            int64_t lds, typename Element<TYPE>::type* __restrict__ out, int64_t ldo, int64_t rows,
-                            unsigned per_row, unsigned rows_per_block) {
+    mxfp4_dequantize_kernel(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds,
+                            typename Element<TYPE>::type* out, int64_t ldo, int64_t rows, unsigned per_row,
+                            unsigned rows_per_block) {
     ptx::let_next_grid_start();
     ptx::wait_for_earlier_grids();
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block;

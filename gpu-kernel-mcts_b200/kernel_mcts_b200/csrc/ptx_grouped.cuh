@@ -11,7 +11,10 @@ namespace ptx {
 // Programmatic dependent launch.  wait_for_earlier_grids returns once the
 // grids before this one in the stream have finished and their writes are
 // visible (at once where the launch did not ask for overlap); every access of
-// global memory comes after it.  let_next_grid_start allows the next grid's
+// global memory comes after it, and is a plain one: read-only loads (__ldg,
+// const __restrict__ parameters) are for data that nothing writes while the
+// kernel runs, and the grid before may still be writing it when this one
+// starts.  let_next_grid_start allows the next grid's
 // blocks onto SMs that have room for them, up to their own wait.
 __device__ __forceinline__ void wait_for_earlier_grids() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
