@@ -11,7 +11,7 @@ import ctypes
 import threading
 from pathlib import Path
 
-from .build import LIBRARY, TORCH_CALLS
+from .build import LIBRARY, TORCH_CALLS, torch_and_python, torch_calls_built_for
 
 KMCTS_OK = 0
 KMCTS_EHANDLE = 1
@@ -282,6 +282,11 @@ def load_torch_calls():
             if not TORCH_CALLS.exists():
                 raise NativeLibraryError(
                     f"{TORCH_CALLS} is not built; run kernel_mcts_b200.build.build_all() (g++, torch headers)"
+                )
+            built_for, here = torch_calls_built_for(), torch_and_python()
+            if built_for not in (None, here):
+                raise NativeLibraryError(
+                    f"{TORCH_CALLS} was built for {built_for}, this is {here}; run kernel_mcts_b200.build.build_all()"
                 )
             spec = importlib.util.spec_from_file_location("kmcts_torch_calls", TORCH_CALLS)
             try:

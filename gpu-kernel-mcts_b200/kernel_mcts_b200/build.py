@@ -13,6 +13,7 @@ sources.
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -30,6 +31,7 @@ OBJ_DIR = LIB_DIR / "obj"
 LIBRARY = LIB_DIR / "libkmcts_gemm_sm100.so"
 HARNESS = LIB_DIR / "kmcts_bf16_eval"
 TORCH_CALLS = LIB_DIR / "kmcts_torch_calls.so"
+TORCH_CALLS_BUILT_FOR = LIB_DIR / "kmcts_torch_calls.built_for"  # torch_and_python() at the time
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = ["-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}"]
@@ -122,6 +124,15 @@ def build_harness(verbose: bool = False) -> Path:
     return HARNESS
 
 
+def torch_and_python() -> str:
+    """What a module built against torch's C++ headers depends on."""
+    return f"torch {importlib.metadata.version('torch')}, {sys.implementation.cache_tag}"
+
+
+def torch_calls_built_for() -> str | None:
+    return TORCH_CALLS_BUILT_FOR.read_text() if TORCH_CALLS_BUILT_FOR.exists() else None
+
+
 def build_torch_calls(verbose: bool = False) -> Path:
     """The torch-facing calls: host code only, against this interpreter's torch."""
     import importlib.util
@@ -129,11 +140,12 @@ def build_torch_calls(verbose: bool = False) -> Path:
     lib = build_library(verbose)
     src = CSRC / "torch_calls.cpp"
     headers = (INCLUDE / "kmcts_grouped.h", INCLUDE / "kmcts_gemm.h")
-    if not _stale(TORCH_CALLS, [src, *headers, Path(__file__)]):
-        return TORCH_CALLS
     spec = importlib.util.find_spec("torch")
     if spec is None or spec.origin is None:
         raise RuntimeError("torch not found; the expert-layer calls are built against its headers")
+    target = torch_and_python()
+    if torch_calls_built_for() == target and not _stale(TORCH_CALLS, [src, *headers, Path(__file__)]):
+        return TORCH_CALLS
     torch_dir = Path(spec.origin).parent
     includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
                 Path(sysconfig.get_paths()["include"]), Path(nvcc()).resolve().parent.parent / "include"]
@@ -146,7 +158,9 @@ def build_torch_calls(verbose: bool = False) -> Path:
     ]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
+    TORCH_CALLS_BUILT_FOR.unlink(missing_ok=True)
     _run(cmd)
+    TORCH_CALLS_BUILT_FOR.write_text(target)
     return TORCH_CALLS
 
 

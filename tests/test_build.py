@@ -1,0 +1,57 @@
+"""The build of the torch-facing module, with the compiler replaced."""
+
+from __future__ import annotations
+
+import os
+
+import pytest
+
+from kernel_mcts_b200 import _native, build
+
+
+@pytest.fixture
+def compiled(monkeypatch, tmp_path):
+    """A build that writes to tmp_path and only records the commands; returns them."""
+    commands = []
+
+    def run(command):
+        commands.append(command)
+        build.TORCH_CALLS.write_bytes(b"")
+
+    monkeypatch.setattr(build, "TORCH_CALLS", tmp_path / "calls.so")
+    monkeypatch.setattr(build, "TORCH_CALLS_BUILT_FOR", tmp_path / "calls.built_for")
+    monkeypatch.setattr(build, "build_library", lambda verbose=False: build.LIBRARY)
+    monkeypatch.setattr(build, "_run", run)
+    return commands
+
+
+def test_torch_calls_are_built_again_for_another_torch(compiled, monkeypatch):
+    build.build_torch_calls()
+    assert len(compiled) == 1
+    build.build_torch_calls()
+    assert len(compiled) == 1  # nothing changed
+    monkeypatch.setattr(build.importlib.metadata, "version", lambda name: "99.0")
+    build.build_torch_calls()
+    assert len(compiled) == 2
+    build.build_torch_calls()
+    assert len(compiled) == 2
+
+
+def test_a_failed_build_leaves_no_claim(compiled, monkeypatch):
+    build.build_torch_calls()
+
+    def fail(command):
+        raise RuntimeError("no compiler")
+
+    monkeypatch.setattr(build, "_run", fail)
+    monkeypatch.setattr(build.importlib.metadata, "version", lambda name: "99.0")
+    with pytest.raises(RuntimeError, match="no compiler"):
+        build.build_torch_calls()
+    assert build.torch_calls_built_for() is None and os.path.exists(build.TORCH_CALLS)
+
+
+def test_a_module_of_another_torch_is_not_loaded(monkeypatch):
+    monkeypatch.setattr(_native, "_calls", None)
+    monkeypatch.setattr(_native, "torch_calls_built_for", lambda: "torch 1.0, cpython-38")
+    with pytest.raises(_native.NativeLibraryError, match="was built for torch 1.0"):
+        _native.load_torch_calls()
