@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import concurrent.futures
 import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -124,6 +125,16 @@ def build_harness(verbose: bool = False) -> Path:
     return HARNESS
 
 
+def torch_dir() -> Path | None:
+    """The installed torch, if it has C++ headers and was built with CUDA."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        return None
+    found = Path(spec.origin).parent
+    needed = ("include/c10/cuda/CUDAStream.h", "include/torch/csrc/utils/pybind.h", "lib/libc10_cuda.so")
+    return found if all((found / name).exists() for name in needed) else None
+
+
 def torch_and_python() -> str:
     """What a module built against torch's C++ headers depends on."""
     return f"torch {importlib.metadata.version('torch')}, {sys.implementation.cache_tag}"
@@ -135,24 +146,21 @@ def torch_calls_built_for() -> str | None:
 
 def build_torch_calls(verbose: bool = False) -> Path:
     """The torch-facing calls: host code only, against this interpreter's torch."""
-    import importlib.util
-
     lib = build_library(verbose)
     src = CSRC / "torch_calls.cpp"
     headers = (INCLUDE / "kmcts_grouped.h", INCLUDE / "kmcts_gemm.h")
-    spec = importlib.util.find_spec("torch")
-    if spec is None or spec.origin is None:
-        raise RuntimeError("torch not found; the expert-layer calls are built against its headers")
+    torch = torch_dir()
+    if torch is None:
+        raise RuntimeError("no torch with CUDA and C++ headers; the expert-layer calls are built against them")
     target = torch_and_python()
     if torch_calls_built_for() == target and not _stale(TORCH_CALLS, [src, *headers, Path(__file__)]):
         return TORCH_CALLS
-    torch_dir = Path(spec.origin).parent
-    includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
+    includes = [torch / "include", torch / "include" / "torch" / "csrc" / "api" / "include",
                 Path(sysconfig.get_paths()["include"]), Path(nvcc()).resolve().parent.parent / "include"]
     cmd = [
         shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{INCLUDE}",
         *(arg for path in includes for arg in ("-isystem", str(path))), str(src), "-o", str(TORCH_CALLS),
-        f"-L{LIB_DIR}", f"-l{lib.stem.removeprefix('lib')}", f"-L{torch_dir / 'lib'}",
+        f"-L{LIB_DIR}", f"-l{lib.stem.removeprefix('lib')}", f"-L{torch / 'lib'}",
         *(f"-l{name}" for name in ("c10", "c10_cuda", "torch", "torch_cpu", "torch_cuda", "torch_python")),
         "-Wl,-rpath,$ORIGIN",
     ]
@@ -165,9 +173,14 @@ def build_torch_calls(verbose: bool = False) -> Path:
 
 
 def build_all(verbose: bool = False) -> None:
+    """Everything that can be built here: the library and the harness need nvcc
+    alone, the torch calls a torch with CUDA and its headers too."""
     build_library(verbose)
     build_harness(verbose)
-    build_torch_calls(verbose)
+    if torch_dir() is not None:
+        build_torch_calls(verbose)
+    else:
+        print("no torch with CUDA and C++ headers: the expert-layer calls on torch tensors are not built", file=sys.stderr)
 
 
 if __name__ == "__main__":

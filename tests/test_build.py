@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import os
+from types import SimpleNamespace
 
 import pytest
 
@@ -55,3 +56,18 @@ def test_a_module_of_another_torch_is_not_loaded(monkeypatch):
     monkeypatch.setattr(_native, "torch_calls_built_for", lambda: "torch 1.0, cpython-38")
     with pytest.raises(_native.NativeLibraryError, match="was built for torch 1.0"):
         _native.load_torch_calls()
+
+
+@pytest.mark.parametrize("torch", ["absent", "without headers"])
+def test_without_torch_the_rest_is_built(compiled, monkeypatch, tmp_path, capsys, torch):
+    built = []
+    monkeypatch.setattr(build, "build_library", lambda verbose=False: built.append("library"))
+    monkeypatch.setattr(build, "build_harness", lambda verbose=False: built.append("harness"))
+    spec = None if torch == "absent" else SimpleNamespace(origin=str(tmp_path / "torch" / "__init__.py"))
+    find_spec = build.importlib.util.find_spec
+    monkeypatch.setattr(build.importlib.util, "find_spec", lambda name: spec if name == "torch" else find_spec(name))
+    build.build_all()
+    assert built == ["library", "harness"] and not compiled
+    assert "not built" in capsys.readouterr().err
+    with pytest.raises(RuntimeError, match="no torch"):
+        build.build_torch_calls()
