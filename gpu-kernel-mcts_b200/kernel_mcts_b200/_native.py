@@ -298,6 +298,18 @@ def load_torch_calls():
         return _calls
 
 
+class _TorchCalls:
+    """The functions of :func:`load_torch_calls`, loaded at their first use."""
+
+    def __getattr__(self, name: str):
+        function = getattr(load_torch_calls(), name)
+        setattr(self, name, function)
+        return function
+
+
+torch_calls = _TorchCalls()
+
+
 def default_config() -> GemmConfig:
     cfg = GemmConfig()
     check(load().kmcts_default_config(ctypes.byref(cfg)), "kmcts_default_config")

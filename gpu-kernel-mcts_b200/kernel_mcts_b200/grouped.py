@@ -26,7 +26,7 @@ KERNELS = {"auto": _native.KERNEL_AUTO, "tcgen05": _native.KERNEL_TCGEN05, "simt
            "pair": _native.KERNEL_GROUPED_PAIR, "split": _native.KERNEL_GROUPED_SPLIT}
 _GRADIENT_KERNELS = {name: KERNELS[name] for name in ("auto", "tcgen05", "simt")}
 
-_calls = _native.load_torch_calls()
+_calls = _native.torch_calls
 
 
 def kernel_code(kernel: str, kernels: dict[str, int] = KERNELS) -> int:

@@ -18,7 +18,7 @@ from .grouped import kernel_code
 
 BLOCK = 32
 
-_calls = _native.load_torch_calls()
+_calls = _native.torch_calls
 
 
 class MXFP4Tensor(NamedTuple):

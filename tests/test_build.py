@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import os
+import subprocess
+import sys
 from types import SimpleNamespace
 
 import pytest
@@ -71,3 +73,26 @@ def test_without_torch_the_rest_is_built(compiled, monkeypatch, tmp_path, capsys
     assert "not built" in capsys.readouterr().err
     with pytest.raises(RuntimeError, match="no torch"):
         build.build_torch_calls()
+
+
+def test_a_missing_module_fails_at_the_first_call(tmp_path):
+    """In a process of its own: the package, its expert-layer modules included,
+    can be imported (and documented, and tested) without the built module."""
+    program = f"""
+import pathlib, sys
+sys.path.insert(0, {str(build.PACKAGE_DIR.parent)!r})
+from kernel_mcts_b200 import _native
+_native.TORCH_CALLS = pathlib.Path({str(tmp_path / "missing.so")!r})
+from kernel_mcts_b200 import grouped, mxfp4
+import torch
+x = torch.zeros(2, 32, dtype=torch.bfloat16)
+for call in (lambda: grouped.grouped_linear(x, x, x), lambda: mxfp4.mxfp4_quantize(x)):
+    try:
+        call()
+    except _native.NativeLibraryError as error:
+        assert "not built" in str(error)
+    else:
+        raise SystemExit("the call did not fail")
+"""
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
