@@ -137,7 +137,13 @@ def torch_dir() -> Path | None:
 
 def torch_and_python() -> str:
     """What a module built against torch's C++ headers depends on."""
-    return f"torch {importlib.metadata.version('torch')}, {sys.implementation.cache_tag}"
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:  # a tree on the path, not an installed package
+        import torch
+
+        version = torch.__version__
+    return f"torch {version}, {sys.implementation.cache_tag}"
 
 
 def torch_calls_built_for() -> str | None:

@@ -8,6 +8,7 @@ import sys
 from types import SimpleNamespace
 
 import pytest
+import torch
 
 from kernel_mcts_b200 import _native, build
 
@@ -40,6 +41,14 @@ def test_torch_calls_are_built_again_for_another_torch(compiled, monkeypatch):
     assert len(compiled) == 2
 
 
+def test_a_torch_without_metadata_tells_its_version(monkeypatch):
+    def missing(name):
+        raise build.importlib.metadata.PackageNotFoundError(name)
+
+    monkeypatch.setattr(build.importlib.metadata, "version", missing)
+    assert torch.__version__ in build.torch_and_python()
+
+
 def test_a_failed_build_leaves_no_claim(compiled, monkeypatch):
     build.build_torch_calls()
 
@@ -60,12 +69,12 @@ def test_a_module_of_another_torch_is_not_loaded(monkeypatch):
         _native.load_torch_calls()
 
 
-@pytest.mark.parametrize("torch", ["absent", "without headers"])
-def test_without_torch_the_rest_is_built(compiled, monkeypatch, tmp_path, capsys, torch):
+@pytest.mark.parametrize("which", ["absent", "without headers"])
+def test_without_torch_the_rest_is_built(compiled, monkeypatch, tmp_path, capsys, which):
     built = []
     monkeypatch.setattr(build, "build_library", lambda verbose=False: built.append("library"))
     monkeypatch.setattr(build, "build_harness", lambda verbose=False: built.append("harness"))
-    spec = None if torch == "absent" else SimpleNamespace(origin=str(tmp_path / "torch" / "__init__.py"))
+    spec = None if which == "absent" else SimpleNamespace(origin=str(tmp_path / "torch" / "__init__.py"))
     find_spec = build.importlib.util.find_spec
     monkeypatch.setattr(build.importlib.util, "find_spec", lambda name: spec if name == "torch" else find_spec(name))
     build.build_all()
