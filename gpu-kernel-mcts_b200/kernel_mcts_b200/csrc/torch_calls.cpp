@@ -216,7 +216,9 @@ class GroupedLinear : public torch::autograd::Function<GroupedLinear> {
 public:
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& ends,
                           int64_t layout) {
-        ctx->save_for_backward({x, w, ends});
+        // The gradient of each needs the other: with a frozen weight the
+        // activations may go, and the other way round.
+        ctx->save_for_backward({w.requires_grad() ? x : Tensor(), x.requires_grad() ? w : Tensor(), ends});
         ctx->saved_data["layout"] = layout;
         return grouped_gemm(x, w, ends, std::nullopt, i32(layout), KMCTS_KERNEL_AUTO, std::nullopt);
     }
