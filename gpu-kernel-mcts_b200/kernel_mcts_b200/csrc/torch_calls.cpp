@@ -135,6 +135,12 @@ void* current_stream(int device) {
     return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
 }
 
+// The caller's tensor has been written: autograd then notices where it was
+// saved for a backward pass.  (Inference tensors count no versions.)
+void mark_written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int i32(int64_t v) { return static_cast<int>(v); }
 
 // ------------------------------------------------------------------- grouped
@@ -166,6 +172,7 @@ Tensor grouped_gemm(const Tensor& x, const Tensor& w, const Tensor& ends, const 
                                        i32(n), i32(k), out ? 0 : KMCTS_GROUPED_ZERO_REST, kernel, current_stream(device),
                                        status_ptr),
                "kmcts_bf16_grouped_gemm");
+    if (out) mark_written(y);
     return y;
 }
 
@@ -202,6 +209,7 @@ Tensor grouped_gemm_wgrad(const Tensor& dy, const Tensor& x, const Tensor& ends,
                                         accumulate, ends.const_data_ptr<int>(), groups, i32(rows), i32(n), i32(k),
                                         kernel, current_stream(device), status_ptr),
                "kmcts_bf16_grouped_wgrad");
+    if (out) mark_written(dw);
     return dw;
 }
 
@@ -319,6 +327,7 @@ std::tuple<Tensor, Tensor> mxfp4_quantize(const Tensor& x, const std::optional<T
                                     strides.codes, scale_rows.mutable_data_ptr(), strides.scales, rows, i32(k),
                                     current_stream(device)),
                "kmcts_mxfp4_quantize");
+    if (out_codes) mark_written(codes), mark_written(scales);
     return {codes, scales};
 }
 
@@ -353,6 +362,7 @@ Tensor mxfp4_dequantize(const Tensor& codes, const Tensor& scales, const std::op
                                       value_rows.mutable_data_ptr(), element_code(type), ldo, rows, i32(k),
                                       current_stream(device)),
                "kmcts_mxfp4_dequantize");
+    if (out) mark_written(values);
     return values;
 }
 
@@ -388,6 +398,7 @@ Tensor mxfp4_gemm(const Tensor& a, const Tensor& a_scales, const Tensor& b, cons
                                 ends ? ends->const_data_ptr<int>() : nullptr, groups, i32(rows), i32(n), i32(k),
                                 out ? 0 : KMCTS_GROUPED_ZERO_REST, kernel, current_stream(device), status_ptr),
                "kmcts_mxfp4_gemm");
+    if (out) mark_written(y);
     return y;
 }
 

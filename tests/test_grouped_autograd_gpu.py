@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from kernel_mcts_b200 import grouped
+from kernel_mcts_b200 import grouped, mxfp4
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,44 @@ def test_only_what_the_backward_pass_reads_is_kept(cuda_device, frozen):
         del w
     assert before - torch.cuda.memory_allocated() == 16 << 20
     y.sum().backward()
+
+
+def writers():
+    """Each call that writes into the caller's tensors: those, and the call."""
+    x, w, ends = operands(64, 32, 64)
+    q = mxfp4.mxfp4_quantize(x)
+    y, dw = torch.zeros(64, 32, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 32, 64, device="cuda")
+    back = torch.zeros(64, 64, dtype=torch.bfloat16, device="cuda")
+    into = mxfp4.MXFP4Tensor(torch.zeros_like(q.codes), torch.zeros_like(q.scales))
+    return {
+        "grouped_gemm": ([y], lambda: grouped.grouped_gemm(x, w, ends, y)),
+        "grouped_gemm_wgrad": ([dw], lambda: grouped.grouped_gemm_wgrad(x[:, :32], x, ends, dw, accumulate=True)),
+        "mxfp4_quantize": (into, lambda: mxfp4.mxfp4_quantize(x, into)),
+        "mxfp4_dequantize": ([back], lambda: mxfp4.mxfp4_dequantize(q, back)),
+        "mxfp4_gemm": ([y], lambda: mxfp4.mxfp4_gemm(q, mxfp4.mxfp4_quantize(w[0]), out=y)),
+    }
+
+
+@pytest.mark.parametrize("name", ["grouped_gemm", "grouped_gemm_wgrad", "mxfp4_quantize", "mxfp4_dequantize", "mxfp4_gemm"])
+def test_a_write_into_the_callers_tensor_counts_as_one(cuda_device, name):
+    tensors, call = writers()[name]
+    before = [t._version for t in tensors]
+    call()
+    assert all(t._version > v for t, v in zip(tensors, before))
+    with torch.inference_mode():
+        tensors, call = writers()[name]  # inference tensors, which count no versions
+        call()
+
+
+def test_a_saved_tensor_that_a_call_overwrites_is_noticed(cuda_device):
+    x, w, ends = operands(64, 32, 64)
+    y = torch.ones(64, 32, dtype=torch.bfloat16, device="cuda")
+    scale = torch.ones(64, 32, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    loss = (scale * y).sum()  # keeps y
+    grouped.grouped_gemm(x, w, ends, y[:, :32])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    kept = grouped.grouped_linear(x.requires_grad_() * 1, w.requires_grad_() * 1, ends)
+    ends.copy_(ends)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.sum().backward()
