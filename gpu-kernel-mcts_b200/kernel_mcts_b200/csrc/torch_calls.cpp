@@ -135,6 +135,13 @@ void* current_stream(int device) {
     return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
 }
 
+// The calls are not recorded by autograd, so what computed the tensor's earlier
+// values would get a gradient for the ones written over them.
+void check_writable(const char* name, const Tensor& t) {
+    if (at::GradMode::is_enabled() && t.requires_grad())
+        throw py::value_error(text(name, " must not require a gradient (write it under torch.no_grad())"));
+}
+
 // The caller's tensor has been written: autograd then notices where it was
 // saved for a backward pass.  (Inference tensors count no versions.)
 void mark_written(const Tensor& t) {
@@ -162,6 +169,7 @@ Tensor grouped_gemm(const Tensor& x, const Tensor& w, const Tensor& ends, const 
     int64_t ldy = n;
     if (out) {
         y = *out;
+        check_writable("out", y);
         ldy = check_rows("out", y, 2, {ScalarType::BFloat16}, device, 8);
         check_shape("out", y, {rows, n});
     } else {
@@ -197,6 +205,7 @@ Tensor grouped_gemm_wgrad(const Tensor& dy, const Tensor& x, const Tensor& ends,
     int64_t ldo = k, group_stride = n * k;
     if (out) {
         dw = *out;
+        check_writable("out", dw);
         ldo = check_rows("out", dw, 3, {type}, device, 8);
         check_shape("out", dw, {groups, n, k});
         group_stride = groups > 1 ? dw.stride(0) : n * ldo;
@@ -352,6 +361,7 @@ Tensor mxfp4_dequantize(const Tensor& codes, const Tensor& scales, const std::op
     int64_t ldo = k;
     if (out) {
         values = *out;
+        check_writable("out", values);
         check_shape("out", values, shape);
         value_rows = as_rows("out", values);
         ldo = check_rows("out", value_rows, 2, {type}, device, kBlock);
@@ -387,6 +397,7 @@ Tensor mxfp4_gemm(const Tensor& a, const Tensor& a_scales, const Tensor& b, cons
     int64_t ldy = n;
     if (out) {
         y = *out;
+        check_writable("out", y);
         ldy = check_rows("out", y, 2, {ScalarType::BFloat16}, device, 8);
         check_shape("out", y, {rows, n});
     } else {

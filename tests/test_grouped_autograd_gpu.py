@@ -76,3 +76,16 @@ def test_a_saved_tensor_that_a_call_overwrites_is_noticed(cuda_device):
     ends.copy_(ends)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         kept.sum().backward()
+
+
+@pytest.mark.parametrize("name", ["grouped_gemm", "grouped_gemm_wgrad", "mxfp4_dequantize", "mxfp4_gemm"])
+def test_results_that_require_a_gradient_are_not_written(cuda_device, name):
+    """Into a value that the autograd graph computed, or a leaf of it."""
+    tensors, call = writers()[name]
+    tensors[0].requires_grad_()
+    with pytest.raises(ValueError, match="must not require a gradient"):
+        call()
+    assert (tensors[0] == 0).all()
+    with torch.no_grad():
+        call()
+    assert not (tensors[0] == 0).all()
