@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(kThreads) grouped_wgrad_simt(WgradArgs p) {
     for (GridWalk walk(0, table.tiles(), blockIdx.x, gridDim.x); walk.more(); walk.next()) {
         const int t = static_cast<int>(walk.at);
         const int e = t / per_group;
+        if (p.accumulate && table.row[e + 1] == table.row[e]) continue;  // adds nothing: -0.0 + 0.0 is 0.0
         const int n0 = t % per_group / tiles_k * kTile, k0 = t % tiles_k * kTile;
         const int rows = min(kTile, p.n - n0), cols = min(kTile, p.k - k0);
         const int64_t t0 = table.row[e];

@@ -78,8 +78,8 @@ def grouped_gemm_wgrad(
 
     The result is ``dtype`` (bfloat16 by default, or float32) or ``out``'s type.
     ``accumulate`` adds to a float32 ``out``, as for a main gradient kept over
-    several micro-batches (sums below ``2^-126`` become zero); an empty group
-    then leaves its part as it was, and is zeros otherwise.
+    several micro-batches; an empty group then leaves its part as it was, and
+    is zeros otherwise.
     """
     args = (dy, x, ends, out, dtype, accumulate, kernel_code(kernel, _GRADIENT_KERNELS), status)
     if stream is None:

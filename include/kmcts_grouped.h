@@ -61,10 +61,10 @@ int kmcts_bf16_grouped_gemm(const void* X, int64_t ldx, const void* W, int64_t w
 
 /* dW_e = dY_e^T * X_e over the rows of group e: dY is [rows, N], X [rows, K]
  * (BF16), dW_e [N, K] at dW + e * dw_stride in dw_type (KMCTS_TYPE_BF16 or
- * KMCTS_TYPE_FP32), FP32 sums.  accumulate (FP32 only) adds to dW, with sums
- * below 2^-126 flushed to zero; otherwise the gradient of an empty group is
- * zeros.  The tensor-core kernel needs
- * 16-byte aligned pointers and strides that are multiples of 16 bytes. */
+ * KMCTS_TYPE_FP32), FP32 sums.  accumulate (FP32 only) adds each sum to dW with
+ * one rounding, subnormals kept, and leaves an empty group's part as it was;
+ * otherwise the gradient of an empty group is zeros.  The tensor-core kernel
+ * needs 16-byte aligned pointers and strides that are multiples of 16 bytes. */
 int kmcts_bf16_grouped_wgrad(const void* dY, int64_t lddy, const void* X, int64_t ldx, void* dW, int64_t dw_stride,
                              int64_t lddw, int dw_type, int accumulate, const int32_t* ends, int groups, int rows,
                              int N, int K, int kernel, void* stream, int* device_status);
