@@ -209,7 +209,10 @@ Tensor grouped_gemm_wgrad(const Tensor& dy, const Tensor& x, const Tensor& ends,
         ldo = check_rows("out", dw, 3, {type}, device, 8);
         check_shape("out", dw, {groups, n, k});
         group_stride = groups > 1 ? dw.stride(0) : n * ldo;
-        if (groups > 1 && n > 0 && group_stride < (n - 1) * ldo + k) throw py::value_error("out has overlapping groups");
+        // Groups one behind the other, or side by side in every row.
+        if (groups > 1 && n > 0 && group_stride < (n - 1) * ldo + k &&
+            (group_stride < k || (n > 1 && ldo < (groups - 1) * group_stride + k)))
+            throw py::value_error("out has overlapping groups");
     } else {
         dw = empty({groups, n, k}, type, device);
     }

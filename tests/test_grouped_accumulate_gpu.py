@@ -48,3 +48,32 @@ def test_accumulate_over_no_rows_changes_nothing(cuda_device, kernel):
     grouped.grouped_gemm_wgrad(none, none, torch.zeros(2, dtype=torch.int32, device="cuda"), main, accumulate=True,
                                kernel=kernel)
     assert torch.equal(main.view(torch.int32), before.view(torch.int32))
+
+
+@pytest.mark.parametrize("kernel", ["tcgen05", "simt"])
+@pytest.mark.parametrize("dtype,accumulate", [(torch.bfloat16, False), (torch.float32, False), (torch.float32, True)])
+def test_groups_side_by_side_in_every_row(cuda_device, kernel, dtype, accumulate):
+    """A main gradient kept as [N, groups, K]: its groups interleave but share nothing."""
+    counts, n, k = [70, 0, 130], 136, 72
+    gen = torch.Generator().manual_seed(1)
+    dy, x = (torch.randint(-2, 3, (200, c), generator=gen).to(torch.bfloat16).cuda() for c in (n, k))
+    ends = torch.tensor(counts).cumsum(0).to(torch.int32).cuda()
+    store = torch.full((n, 4, k), 3, dtype=dtype, device="cuda")
+    out = store[:, :3].transpose(0, 1)
+    assert out.shape == (3, n, k) and out.stride(0) == k
+    grouped.grouped_gemm_wgrad(dy, x, ends, out, accumulate=accumulate, kernel=kernel)
+    want = torch.stack([dy[:70].double().T @ x[:70].double(), torch.zeros(n, k, device="cuda").double(),
+                        dy[70:].double().T @ x[70:].double()])
+    assert torch.equal(out, (want + (3 if accumulate else 0)).to(dtype))
+    assert (store[:, 3] == 3).all()
+
+
+def test_groups_that_overlap_are_refused(cuda_device):
+    dy, x = torch.zeros(4, 8, dtype=torch.bfloat16, device="cuda"), torch.zeros(4, 16, dtype=torch.bfloat16, device="cuda")
+    ends = torch.tensor([2, 4], dtype=torch.int32, device="cuda")
+    store = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")
+    for strides in ((0, 16, 1), (8, 32, 1), (16, 24, 1), (7 * 16, 16, 1)):
+        with pytest.raises(ValueError, match="overlapping groups"):
+            grouped.grouped_gemm_wgrad(dy, x, ends, store.as_strided((2, 8, 16), strides))
+    for strides in ((16, 32, 1), (128, 16, 1), (7 * 32 + 16, 32, 1)):
+        grouped.grouped_gemm_wgrad(dy, x, ends, store.as_strided((2, 8, 16), strides))
