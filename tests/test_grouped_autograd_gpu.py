@@ -3,8 +3,12 @@ for the backward pass, hooks, and results written into the caller's tensors."""
 
 from __future__ import annotations
 
+import contextlib
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 from kernel_mcts_b200 import grouped, mxfp4
 
@@ -89,3 +93,55 @@ def test_results_that_require_a_gradient_are_not_written(cuda_device, name):
     with torch.no_grad():
         call()
     assert not (tensors[0] == 0).all()
+
+
+def gradients(x, w, ends, dy, around):
+    """(y, dx, dw) of a step within a context, from leaves of its own."""
+    x, w = x.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+    with around:
+        y = grouped.grouped_linear(x, w, ends)
+    y.backward(dy)
+    return y.detach(), x.grad, w.grad
+
+
+def test_saved_tensor_hooks_and_checkpointing(cuda_device):
+    """What is kept may be moved to the host and back, or computed again."""
+    x, w, ends = operands(200, 136, 72)
+    dy = operands(200, 136, 136)[0]
+    plain = gradients(x, w, ends, dy, contextlib.nullcontext())
+    moved = gradients(x, w, ends, dy, torch.autograd.graph.save_on_cpu())
+    assert all(torch.equal(a, b) for a, b in zip(plain, moved))
+    for reentrant in (False, True):
+        x2, w2 = x.clone().requires_grad_(), w.clone().requires_grad_()
+        y = checkpoint(lambda a, b: grouped.grouped_linear(a, b, ends), x2, w2, use_reentrant=reentrant)
+        y.backward(dy)
+        assert all(torch.equal(a, b) for a, b in zip(plain, (y.detach(), x2.grad, w2.grad)))
+
+
+def test_steps_on_two_threads_and_streams(cuda_device):
+    x, w, ends = operands(200, 136, 72)
+    dy = operands(200, 136, 136)[0]
+    plain = gradients(x, w, ends, dy, contextlib.nullcontext())
+    torch.cuda.synchronize()
+
+    def steps(_):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            results = [gradients(x, w, ends, dy, contextlib.nullcontext()) for _ in range(20)]
+        stream.synchronize()
+        return all(torch.equal(a, b) for result in results for a, b in zip(plain, result))
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(steps, range(4)))
+
+
+def test_gradients_of_one_weight_shared_by_all_groups(cuda_device):
+    """An expanded weight's gradient is the sum over the groups."""
+    x, w, ends = operands(200, 136, 72)
+    dy = operands(200, 136, 136)[0]
+    one = w[:1].clone().requires_grad_()
+    y = grouped.grouped_linear(x, one.expand(2, 136, 72), ends)
+    (got,) = torch.autograd.grad(y, one, dy)
+    cut = int(ends[0])
+    parts = [(dy[lo:hi].double().T @ x[lo:hi].double()).to(torch.bfloat16) for lo, hi in ((0, cut), (cut, 200))]
+    assert torch.equal(got[0], parts[0] + parts[1])
