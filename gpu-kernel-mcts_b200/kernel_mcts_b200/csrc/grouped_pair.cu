@@ -21,13 +21,19 @@
 // reads the groups' ends itself and walks the tiles round-robin; nothing is
 // decided on the host.  Every wait is bounded.
 //
-// Bounds and layout, measured on B200 (bursts): forward products run at 1.2 to
-// 1.5 PFLOP/s, the tensor pipe busy 78% of the time, held back by operands
-// from L2 (10 TB/s into the SMs) and by tiles that do not share out evenly over
-// 74 pairs; gradients at 1.1 to 1.4, where short contractions are bound by
-// writing the gradient; MXFP4 at 4.0, bound by L2 likewise (each tile moves 448
-// rows of operands for 256 x 192 outputs).  Longest-tile-first orders would
-// gain 2 to 3% on skewed groups by simulation and are left out.
+// Bounds, measured on two B200 in bursts (graph replays of several calls on
+// operands beyond L2; times elsewhere in this file are taken so, too, before
+// and after the choice at hand).  8192 rows of 4096 x 4096, PFLOP/s: forward
+// products 1.50 to 1.57 with one group, 1.37 to 1.44 with 16 equal ones, 1.22
+// to 1.29 with skewed ones; gradients 1.36 to 1.40, 1.13 to 1.19, 1.07 to 1.13;
+// MXFP4 at 8192^3 3.75 to 4.06.  The tensor pipe is busy 78% of the time, held
+// back by operands from L2 (10 TB/s into the SMs; an MXFP4 tile moves 448 rows
+// of them for 256 x 192 outputs).  Skewed groups' tiles differ in width, and
+// round-robin leaves the longest pair 8 to 12% over an even share (simulated
+// over 40 draws; a shared counter would leave 6%, the widest first 4%).  A
+// product of fewer than 74 tiles leaves pairs idle, and a gradient's
+// contraction is not split: one tile of 8192 rows takes 42 us.  Gradients of a
+// few rows are bound by writing them.
 #include <mutex>
 
 #include "grouped_tiles.cuh"

@@ -85,7 +85,7 @@ __device__ __forceinline__ Tile tile_at(const GroupTable& table, const SplitPara
     out.t0 = first + (in_group - n_blk * tiles_t) * step;
     out.valid = min(step, first + rows - out.t0);
     out.width = round_up(out.valid, 16);
-    // Splits are 1, 2 or 4.
+    // Splits are 2 or 4.
     const int blocks = (p.k + Split<KIND>::kBK - 1) / Split<KIND>::kBK, shift = splits >> 1;
     out.kb0 = static_cast<int>(static_cast<int64_t>(rank) * blocks >> shift);
     out.kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * blocks >> shift);

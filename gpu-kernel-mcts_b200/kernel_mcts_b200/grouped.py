@@ -13,6 +13,11 @@ The weight of group ``e`` is ``w[e]``: ``[N, K]`` for ``w_layout="col"``
 weight of a ``"col"`` product is that product's input gradient,
 :func:`grouped_gemm_wgrad` its weights' gradient, and :func:`grouped_linear`
 ties the three together for autograd.
+
+:func:`grouped_gemm` and :func:`grouped_gemm_wgrad` are not recorded by
+autograd: their results require no gradient, whatever the operands do, and an
+``out`` that requires one is refused while autograd records.  A write into
+``out`` counts as an in-place change.
 """
 
 from __future__ import annotations
@@ -91,7 +96,9 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, *, w_la
     """Differentiable ``grouped_gemm(x, w, ends, w_layout=w_layout)``.
 
     The gradients of ``x`` and ``w`` are bfloat16; ``x``'s is zero in rows
-    behind the last group.  Once differentiable.  As with any torch function, a
+    behind the last group.  Of ``x`` and ``w`` only what the wanted gradients
+    read is kept.  Once differentiable: a backward pass with ``create_graph=True``
+    is refused.  As with any torch function, a
     backward pass may be captured into a CUDA graph only while no autograd
     graph of the same leaves from outside the capture is alive."""
     return _calls.grouped_linear(x, w, ends, layout_code(w_layout))

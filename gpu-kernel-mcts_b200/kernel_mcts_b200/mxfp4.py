@@ -5,6 +5,9 @@ An MXFP4 tensor of logical shape ``[..., K]`` is a pair of uint8 tensors:
 half, and ``scales`` ``[..., K/32]``, one E8M0 exponent (``2^(s - 127)``, 255 is
 NaN) for each block of 32 elements.  Both may be views with strided rows, and
 may be given as torch's ``float4_e2m1fn_x2`` and ``float8_e8m0fnu`` types.
+
+The calls are not recorded by autograd: results require no gradient, and an
+``out`` that requires one is refused while autograd records.
 """
 
 from __future__ import annotations

@@ -17,7 +17,9 @@
  * innermost dimension is contiguous.  Calls are asynchronous on `stream` and
  * run on the current device; they keep nothing between calls and use no
  * workspace, so calls on different streams, and graphs that captured them,
- * may overlap.  device_status is as for kmcts_bf16_gemm_ex.
+ * may overlap.  device_status is as for kmcts_bf16_gemm_ex: a wait that gives
+ * up (after two seconds, and ten microseconds more for each stage of K or of a
+ * group's rows that one CTA walks through) sets it and leaves results unwritten.
  *
  * Returns KMCTS_OK, KMCTS_EINVAL (pointers, sizes, strides, groups),
  * KMCTS_ENOTSUP (the requested kernel cannot run these arguments) or
