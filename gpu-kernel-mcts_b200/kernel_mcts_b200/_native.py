@@ -302,6 +302,8 @@ class _TorchCalls:
     """The functions of :func:`load_torch_calls`, loaded at their first use."""
 
     def __getattr__(self, name: str):
+        if name.startswith("__"):  # asked by inspect, copy and the like, which want no library loaded
+            raise AttributeError(name)
         function = getattr(load_torch_calls(), name)
         setattr(self, name, function)
         return function

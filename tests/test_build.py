@@ -94,6 +94,7 @@ from kernel_mcts_b200 import _native
 _native.TORCH_CALLS = pathlib.Path({str(tmp_path / "missing.so")!r})
 from kernel_mcts_b200 import grouped, mxfp4
 import torch
+assert not hasattr(_native.torch_calls, "__wrapped__")  # looking at it loads nothing
 x = torch.zeros(2, 32, dtype=torch.bfloat16)
 for call in (lambda: grouped.grouped_linear(x, x, x), lambda: mxfp4.mxfp4_quantize(x)):
     try:
